@@ -8,12 +8,15 @@ lives in ``libweaver_cuda.so`` (hand-written CUDA for sm_100a, C ABI in
 ``include/weaver_cuda.h``); this package is its Python host API.
 """
 from ._native import WeaverError, library_path
+from .prefix import PrefixPlan
+from .rope import Rope, rope_frequencies, token_slots
 from .types import (BLOCK_SIZE, REF_MASK, SPARSE_CODE_DTYPE, SPARSITY_K, FabricRegions, LoomDescriptor,
                     ModelDims, Persona, WeaverParams, sparse_code_zero)
 from .weaver import DecodeOutput, WeaverEngine, WeaverPlan, distill, merge_partials, merge_partials_packed
 
 __all__ = [
     "BLOCK_SIZE", "REF_MASK", "SPARSE_CODE_DTYPE", "SPARSITY_K", "DecodeOutput", "FabricRegions",
-    "LoomDescriptor", "ModelDims", "Persona", "WeaverEngine", "WeaverError", "WeaverParams", "WeaverPlan",
-    "distill", "library_path", "merge_partials", "merge_partials_packed", "sparse_code_zero",
+    "LoomDescriptor", "ModelDims", "Persona", "PrefixPlan", "Rope", "WeaverEngine", "WeaverError", "WeaverParams",
+    "WeaverPlan", "distill", "library_path", "merge_partials", "merge_partials_packed", "rope_frequencies",
+    "sparse_code_zero", "token_slots",
 ]

@@ -20,6 +20,8 @@ STATUS_NAMES = {
     6: "WEAVER_ERR_NO_DEVICE", 7: "WEAVER_ERR_TIMEOUT", 8: "WEAVER_ERR_CAPACITY",
 }
 FLAG_CAUSAL, FLAG_QLATENT_INPUT, FLAG_PARTIALS = 1, 2, 4
+F16, BF16 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 
 class SparseCodeC(ctypes.Structure):
@@ -76,6 +78,37 @@ class ViewsC(ctypes.Structure):
                 ("out", c_void_p), ("part_m", c_void_p), ("part_l", c_void_p), ("part_o", c_void_p)]
 
 
+class RopeConfigC(ctypes.Structure):
+    _fields_ = [("head_dim", c_u32), ("rot_dim", c_u32), ("layout", c_u32), ("amplitude", c_float),
+                ("inv_freq", c_void_p)]
+
+
+class RopeViewsC(ctypes.Structure):
+    _fields_ = [("n_tokens", c_u32), ("q_heads", c_u32), ("kv_heads", c_u32), ("dtype", c_u32),
+                ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+                ("q_token_stride", c_u64), ("q_head_stride", c_u64), ("k_token_stride", c_u64),
+                ("k_head_stride", c_u64), ("v_token_stride", c_u64), ("v_head_stride", c_u64),
+                ("positions", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float),
+                ("_pad", c_u32), ("q_out", c_void_p), ("k_out", c_void_p), ("q_out_token_stride", c_u64),
+                ("q_out_head_stride", c_u64), ("k_out_token_stride", c_u64), ("k_out_head_stride", c_u64),
+                ("slots", c_void_p), ("hot_k", c_void_p), ("hot_v", c_void_p), ("hot_pool_blocks", c_u64),
+                ("bad_flag", c_void_p)]
+
+
+class PrefixShapeC(ctypes.Structure):
+    _fields_ = [("num_groups", c_u32), ("num_seqs", c_u32), ("q_heads", c_u32), ("kv_heads", c_u32),
+                ("head_dim", c_u32), ("scale", c_float), ("flags", c_u32), ("_pad", c_u32)]
+
+
+class PrefixViewsC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("hot_k", c_void_p), ("hot_v", c_void_p), ("hot_pool_blocks", c_u64),
+                ("prefix_refs", c_void_p), ("suffix_refs", c_void_p), ("prefix_lens", c_void_p),
+                ("suffix_lens", c_void_p), ("out", c_void_p), ("part_m", c_void_p), ("part_l", c_void_p),
+                ("part_o", c_void_p)]
+
+
+assert ctypes.sizeof(RopeConfigC) == 24 and ctypes.sizeof(RopeViewsC) == 208
+assert ctypes.sizeof(PrefixShapeC) == 32 and ctypes.sizeof(PrefixViewsC) == 96
 assert ctypes.sizeof(SparseCodeC) == 16 and ctypes.sizeof(WeaverParamsC) == 48
 assert ctypes.sizeof(LoomDescriptorC) == 32
 assert ctypes.sizeof(FabricGeometryC) == 48 and ctypes.sizeof(FabricLayerC) == 64
@@ -135,6 +168,16 @@ SIGNATURES = [
                                            c_u32, c_u32, c_void_p]),
     ("weaver_distill_stats", c_int, [c_void_p, c_u32, c_u32, c_u32, c_void_p, c_u32, c_u64, c_void_p, c_void_p,
                                      c_void_p]),
+    ("weaver_rope_create", c_int, [c_void_p, ctypes.POINTER(RopeConfigC), ctypes.POINTER(c_void_p)]),
+    ("weaver_rope_destroy", None, [c_void_p]),
+    ("weaver_rope_rotate", c_int, [c_void_p, ctypes.POINTER(RopeViewsC), c_void_p]),
+    ("weaver_rope_append", c_int, [c_void_p, ctypes.POINTER(RopeViewsC), c_void_p]),
+    ("weaver_prefix_plan_create", c_int, [c_void_p, ctypes.POINTER(PrefixShapeC), c_void_p, c_void_p, c_void_p,
+                                          c_void_p, ctypes.POINTER(c_void_p)]),
+    ("weaver_prefix_plan_destroy", None, [c_void_p]),
+    ("weaver_prefix_run", c_int, [c_void_p, ctypes.POINTER(PrefixViewsC), c_void_p]),
+    ("weaver_prefix_plan_kernel_count", c_int, [c_void_p]),
+    ("weaver_prefix_plan_status", c_int, [c_void_p]),
 ]
 
 _lib = None

@@ -5,9 +5,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
+#include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1834,3 +1838,341 @@ int weaver_loom_page_tables(const weaver_device_fabric* f, const weaver_loom_des
 
 }  // extern "C"
 
+// ---- position rotation and the append (ops.metal:107-160, inference.rs:504-562) ----
+
+struct weaver_rope {
+    int device = 0;
+    RopeArgs base{};
+};
+
+namespace {
+
+// Makes `device` current for one call and puts the caller's device back.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t err;
+    explicit DeviceScope(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// An output [T][H][D] whose elements do not overlap.
+bool disjoint_rows(uint64_t T, uint64_t H, uint64_t D, uint64_t ts, uint64_t hs) {
+    if (T == 0 || H == 0) return true;
+    const uint64_t token = (H - 1) * hs + D, head = (T - 1) * ts + D;
+    const bool heads_inside = (H == 1 || hs >= D) && (T == 1 || ts >= token);
+    const bool tokens_inside = (T == 1 || ts >= D) && (H == 1 || hs >= head);
+    return heads_inside || tokens_inside;
+}
+
+int rope_output(const char* name, const void* in, uint64_t in_ts, uint64_t in_hs, const void* out, uint64_t ts,
+                uint64_t hs, uint64_t T, uint64_t H, uint64_t D) {
+    if (!in || !out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s or its output is null", name);
+    if (!aligned16(in) || !aligned16(out) || in_ts % 8 || in_hs % 8 || ts % 8 || hs % 8)
+        return fail(WEAVER_ERR_MISALIGNED, "%s rows not 16-byte aligned", name);
+    if (!disjoint_rows(T, H, D, ts, hs)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "rows of %s's output overlap", name);
+    const char* i0 = static_cast<const char*>(in);
+    const char* o0 = static_cast<const char*>(out);
+    if (T && H && !(in == out && in_ts == ts && in_hs == hs)) {  // the same rows, or none in common
+        const char* i1 = i0 + 2 * ((T - 1) * in_ts + (H - 1) * in_hs + D);
+        const char* o1 = o0 + 2 * ((T - 1) * ts + (H - 1) * hs + D);
+        if (i0 < o1 && o0 < i1)
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s's output overlaps it with other strides", name);
+    }
+    return WEAVER_OK;
+}
+
+int rope_run(weaver_rope* rope, const weaver_rope_views* v, void* stream, bool append) {
+    if (!rope || !v) return fail(WEAVER_ERR_INVALID_ARGUMENT, "null argument");
+    RopeArgs a = rope->base;
+    const uint64_t T = v->n_tokens, D = a.D;
+    if (T == 0) return WEAVER_OK;
+    if (v->dtype != WEAVER_F16 && v->dtype != WEAVER_BF16)
+        return fail(WEAVER_ERR_UNSUPPORTED, "dtype %u (f16 and bf16)", v->dtype);
+    if (v->q_heads == 0 && v->kv_heads == 0) return fail(WEAVER_ERR_INVALID_ARGUMENT, "no heads");
+    if (v->q_heads > 65535 || v->kv_heads > 65535 || T > 0x7FFFFFFFull)
+        return fail(WEAVER_ERR_CAPACITY, "%u + %u heads, %u tokens", v->q_heads, v->kv_heads, v->n_tokens);
+    if (!v->positions || (reinterpret_cast<uintptr_t>(v->positions) & 3u))
+        return fail(WEAVER_ERR_INVALID_ARGUMENT, "positions null or misaligned");
+    if ((v->q_weight || v->k_weight) && !(v->eps >= 0.0f && std::isfinite(v->eps)))
+        return fail(WEAVER_ERR_INVALID_ARGUMENT, "eps %g", static_cast<double>(v->eps));
+    if (!aligned16(v->q_weight) || !aligned16(v->k_weight)) return fail(WEAVER_ERR_MISALIGNED, "weights not 16-byte aligned");
+    int rc;
+    if (v->q_heads && (rc = rope_output("q", v->q, v->q_token_stride, v->q_head_stride, v->q_out, v->q_out_token_stride,
+                                        v->q_out_head_stride, T, v->q_heads, D)))
+        return rc;
+    if (append) {
+        if (!v->kv_heads || !v->k || !v->hot_k || !v->slots || !v->bad_flag)
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "append needs k, hot_k, slots and bad_flag");
+        if (!v->v != !v->hot_v) return fail(WEAVER_ERR_INVALID_ARGUMENT, "v and hot_v come together");
+        if (v->hot_k == v->hot_v)
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_v is hot_k: pass v and hot_v null for a pool shared by K and V");
+        if (v->hot_pool_blocks == 0 || v->hot_pool_blocks > (1ull << 31))
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_pool_blocks %llu", (unsigned long long)v->hot_pool_blocks);
+        if (!aligned16(v->k) || !aligned16(v->v) || !aligned16(v->hot_k) || !aligned16(v->hot_v) ||
+            v->k_token_stride % 8 || v->k_head_stride % 8 || (v->v && (v->v_token_stride % 8 || v->v_head_stride % 8)))
+            return fail(WEAVER_ERR_MISALIGNED, "k, v or the pool not 16-byte aligned");
+        if ((reinterpret_cast<uintptr_t>(v->slots) & 7u) || (reinterpret_cast<uintptr_t>(v->bad_flag) & 3u))
+            return fail(WEAVER_ERR_MISALIGNED, "slots or bad_flag misaligned");
+    } else if (v->kv_heads && (rc = rope_output("k", v->k, v->k_token_stride, v->k_head_stride, v->k_out,
+                                                v->k_out_token_stride, v->k_out_head_stride, T, v->kv_heads, D))) {
+        return rc;
+    }
+    a.q = v->q;
+    a.k = v->k;
+    a.v = append ? v->v : nullptr;
+    a.q_weight = v->q_heads ? v->q_weight : nullptr;
+    a.k_weight = v->kv_heads ? v->k_weight : nullptr;
+    a.q_out = v->q_out;
+    a.k_out = v->k_out;
+    a.hot_k = v->hot_k;
+    a.hot_v = v->hot_v;
+    a.q_ts = v->q_token_stride, a.q_hs = v->q_head_stride;
+    a.k_ts = v->k_token_stride, a.k_hs = v->k_head_stride;
+    a.v_ts = v->v_token_stride, a.v_hs = v->v_head_stride;
+    a.qo_ts = v->q_out_token_stride, a.qo_hs = v->q_out_head_stride;
+    a.ko_ts = v->k_out_token_stride, a.ko_hs = v->k_out_head_stride;
+    a.positions = v->positions;
+    a.slots = v->slots;
+    a.bad = v->bad_flag;
+    a.pool_rows = v->hot_pool_blocks * kBlock;
+    a.T = v->n_tokens;
+    a.Hq = v->q_heads;
+    a.Hkv = v->kv_heads;
+    a.bf16 = v->dtype == WEAVER_BF16;
+    a.eps = v->eps;
+    DeviceScope dev(rope->device);
+    WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
+    WEAVER_CUDA_TRY(launch_rope(a, append, static_cast<cudaStream_t>(stream)), append ? "append launch" : "rotation launch");
+    return WEAVER_OK;
+}
+
+}  // namespace
+
+struct weaver_prefix_plan {
+    int device = 0;
+    weaver_prefix_shape shape{};
+    PrefixArgs base{};
+    void* arena = nullptr;
+    uint32_t n_items16 = 0;
+    bool merge = false;
+    uint64_t n_prefix_pages = 0, n_suffix_pages = 0;
+    cudaStream_t last_stream = nullptr;
+};
+
+extern "C" {
+
+int weaver_rope_create(weaver_engine* eng, const weaver_rope_config* c, weaver_rope** out) {
+    if (!eng || !c || !out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "null argument to weaver_rope_create");
+    *out = nullptr;
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(WEAVER_ERR_UNSUPPORTED, "head_dim %u (built for 64 and 128)", c->head_dim);
+    if (c->rot_dim % 16 || c->rot_dim > c->head_dim)
+        return fail(WEAVER_ERR_UNSUPPORTED, "rot_dim %u (a multiple of 16 up to head_dim)", c->rot_dim);
+    if (c->layout != WEAVER_ROPE_HALF && c->layout != WEAVER_ROPE_INTERLEAVED)
+        return fail(WEAVER_ERR_INVALID_ARGUMENT, "layout %u", c->layout);
+    if (c->rot_dim && !c->inv_freq) return fail(WEAVER_ERR_INVALID_ARGUMENT, "inv_freq is null");
+    if (!std::isfinite(c->amplitude)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "amplitude is not finite");
+    weaver_rope* r = new (std::nothrow) weaver_rope();
+    if (!r) return fail(WEAVER_ERR_CAPACITY, "out of host memory");
+    r->device = eng->device;
+    r->base.D = c->head_dim;
+    r->base.rot = c->rot_dim;
+    r->base.interleaved = c->layout == WEAVER_ROPE_INTERLEAVED;
+    r->base.amplitude = c->amplitude;
+    for (uint32_t i = 0; i < c->rot_dim / 2; ++i) {
+        if (!std::isfinite(c->inv_freq[i])) {
+            delete r;
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "inv_freq[%u] is not finite", i);
+        }
+        // turns per position modulo one (positions are whole numbers), times 2^64
+        const long double turns = static_cast<long double>(c->inv_freq[i]) / 6.283185307179586476925286766559L;
+        const long double frac = turns - std::floor(turns);
+        const long double scaled = std::ldexp(frac, 64);
+        r->base.freq[i] = scaled >= 18446744073709551615.0L ? 0ull : static_cast<uint64_t>(scaled + 0.5L);
+    }
+    *out = r;
+    return WEAVER_OK;
+}
+
+void weaver_rope_destroy(weaver_rope* rope) { delete rope; }
+
+int weaver_rope_rotate(weaver_rope* rope, const weaver_rope_views* views, void* stream) {
+    return rope_run(rope, views, stream, false);
+}
+
+int weaver_rope_append(weaver_rope* rope, const weaver_rope_views* views, void* stream) {
+    return rope_run(rope, views, stream, true);
+}
+
+// ---- attention for a batch that shares prefixes ---------------------------------
+
+int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh, const uint32_t* q_indptr,
+                              const uint32_t* group_indptr, const uint32_t* prefix_indptr,
+                              const uint32_t* suffix_indptr, weaver_prefix_plan** out) try {
+    if (!eng || !sh || !q_indptr || !group_indptr || !prefix_indptr || !suffix_indptr || !out)
+        return fail(WEAVER_ERR_INVALID_ARGUMENT, "null argument to weaver_prefix_plan_create");
+    *out = nullptr;
+    const uint32_t NG = sh->num_groups, B = sh->num_seqs, Hq = sh->q_heads, Hkv = sh->kv_heads, D = sh->head_dim;
+    if (NG == 0 || B == 0 || Hq == 0 || Hkv == 0) return fail(WEAVER_ERR_INVALID_ARGUMENT, "zero dimension in shape");
+    if (Hq % Hkv) return fail(WEAVER_ERR_INVALID_ARGUMENT, "q_heads %u not a multiple of kv_heads %u", Hq, Hkv);
+    if (D != 64 && D != 128) return fail(WEAVER_ERR_UNSUPPORTED, "head_dim %u (built for 64 and 128)", D);
+    if (sh->flags & ~(WEAVER_FLAG_CAUSAL | WEAVER_FLAG_PARTIALS))
+        return fail(WEAVER_ERR_UNSUPPORTED, "flags %u", sh->flags);
+    if (!std::isfinite(sh->scale)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "scale is not finite");
+    if (NG > (1u << 24) || B > (1u << 24) || Hq > 65535)
+        return fail(WEAVER_ERR_CAPACITY, "%u groups, %u sequences, %u heads", NG, B, Hq);
+    if (q_indptr[0] || group_indptr[0] || prefix_indptr[0] || suffix_indptr[0])
+        return fail(WEAVER_ERR_INVALID_ARGUMENT, "indptr[0] must be 0");
+    for (uint32_t g = 0; g < NG; ++g)
+        if (group_indptr[g + 1] < group_indptr[g] || prefix_indptr[g + 1] < prefix_indptr[g])
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "indptr not monotone at group %u", g);
+    if (group_indptr[NG] != B) return fail(WEAVER_ERR_INVALID_ARGUMENT, "the groups hold %u of %u sequences", group_indptr[NG], B);
+    for (uint32_t b = 0; b < B; ++b)
+        if (q_indptr[b + 1] < q_indptr[b] || suffix_indptr[b + 1] < suffix_indptr[b])
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "indptr not monotone at sequence %u", b);
+    // rows, positions and pages are counted in 31 bits
+    if (static_cast<uint64_t>(q_indptr[B]) * Hq >= (1ull << 31)) return fail(WEAVER_ERR_CAPACITY, "%u queries x %u heads", q_indptr[B], Hq);
+    if (prefix_indptr[NG] > (1u << 26) || suffix_indptr[B] > (1u << 26)) return fail(WEAVER_ERR_CAPACITY, "more than 2^26 pages");
+
+    DeviceScope dev(eng->device);
+    WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
+    PrefixGeometry geo{NG, B, Hq, Hkv, D, (sh->flags & WEAVER_FLAG_CAUSAL) != 0, (sh->flags & WEAVER_FLAG_PARTIALS) != 0,
+                       q_indptr, group_indptr, prefix_indptr, suffix_indptr};
+    PrefixTables t;
+    plan_prefix(geo, static_cast<uint32_t>(eng->prop.multiProcessorCount), &t);
+    if (t.items16.size() > 0x7FFFFFFFull || t.tiles.size() > 0x7FFFFFFFull) return fail(WEAVER_ERR_CAPACITY, "too many work items");
+
+    // one allocation: tables, status, partials
+    size_t off = 0;
+    auto place = [&](size_t bytes) {
+        const size_t o = off;
+        off = align_up(off + bytes, 256);
+        return o;
+    };
+    const size_t o_lists = place(t.lists.size() * sizeof(PrefixList)), o_tiles = place(t.tiles.size() * sizeof(PrefixTile)),
+                 o_items = place(t.items16.size() * sizeof(PrefixItem)), o_seq = place(t.tok_seq.size() * 4),
+                 o_group = place(t.seq_group.size() * 4), o_status = place(8), o_ml = place(t.part_rows * sizeof(float2)),
+                 o_o = place(t.part_rows * D * sizeof(float));
+    auto plan = std::unique_ptr<weaver_prefix_plan>(new weaver_prefix_plan());
+    plan->device = eng->device;
+    cudaError_t e = cudaMalloc(&plan->arena, off);
+    if (e != cudaSuccess) return cuda_fail(e, "prefix plan allocation");
+    char* base = static_cast<char*>(plan->arena);
+    auto upload = [&](size_t o, const void* src, size_t bytes) {
+        if (e == cudaSuccess && bytes) e = cudaMemcpy(base + o, src, bytes, cudaMemcpyHostToDevice);
+    };
+    upload(o_lists, t.lists.data(), t.lists.size() * sizeof(PrefixList));
+    upload(o_tiles, t.tiles.data(), t.tiles.size() * sizeof(PrefixTile));
+    upload(o_items, t.items16.data(), t.items16.size() * sizeof(PrefixItem));
+    upload(o_seq, t.tok_seq.data(), t.tok_seq.size() * 4);
+    upload(o_group, t.seq_group.data(), t.seq_group.size() * 4);
+    const uint32_t zero[2] = {0, 0};
+    upload(o_status, zero, sizeof(zero));
+    if (e != cudaSuccess) {
+        cudaFree(plan->arena);
+        return cuda_fail(e, "prefix plan upload");
+    }
+    plan->shape = *sh;
+    plan->n_items16 = static_cast<uint32_t>(t.items16.size());
+    plan->merge = t.needs_merge;
+    plan->n_prefix_pages = prefix_indptr[NG];
+    plan->n_suffix_pages = suffix_indptr[B];
+    PrefixArgs& a = plan->base;
+    a.lists = reinterpret_cast<const PrefixList*>(base + o_lists);
+    a.tiles = reinterpret_cast<const PrefixTile*>(base + o_tiles);
+    a.items = reinterpret_cast<const PrefixItem*>(base + o_items);
+    a.tok_seq = reinterpret_cast<const uint32_t*>(base + o_seq);
+    a.seq_group = reinterpret_cast<const uint32_t*>(base + o_group);
+    a.status = reinterpret_cast<uint32_t*>(base + o_status);
+    a.part_ml = reinterpret_cast<float2*>(base + o_ml);
+    a.part_o = reinterpret_cast<float*>(base + o_o);
+    a.n_groups = NG;
+    a.n_tokens = q_indptr[B];
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.G = Hq / Hkv;
+    a.D = D;
+    a.scale = sh->scale;
+    *out = plan.release();
+    return WEAVER_OK;
+} catch (const std::exception& ex) {
+    return fail(WEAVER_ERR_CAPACITY, "prefix plan: %s", ex.what());
+}
+
+void weaver_prefix_plan_destroy(weaver_prefix_plan* plan) {
+    if (!plan) return;
+    DeviceScope dev(plan->device);
+    cudaFree(plan->arena);
+    delete plan;
+}
+
+int weaver_prefix_plan_kernel_count(const weaver_prefix_plan* plan) {
+    if (!plan) return 0;
+    return (plan->n_items16 ? 1 : 0) + (plan->merge ? 1 : 0);
+}
+
+int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, void* stream) {
+    if (!plan || !v) return fail(WEAVER_ERR_INVALID_ARGUMENT, "null argument to weaver_prefix_run");
+    PrefixArgs a = plan->base;
+    if (a.n_tokens == 0) return WEAVER_OK;
+    if (plan->shape.flags & WEAVER_FLAG_PARTIALS) {
+        if (!v->part_m || !v->part_l || !v->part_o) return fail(WEAVER_ERR_INVALID_ARGUMENT, "partial outputs are null");
+        if (!aligned16(v->part_o) || (reinterpret_cast<uintptr_t>(v->part_m) & 3u) ||
+            (reinterpret_cast<uintptr_t>(v->part_l) & 3u))
+            return fail(WEAVER_ERR_MISALIGNED, "partial outputs misaligned");
+        a.out_m = v->part_m;
+        a.out_l = v->part_l;
+        a.out_o = v->part_o;
+    } else {
+        if (!v->out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "views.out is null");
+        if (!aligned16(v->out)) return fail(WEAVER_ERR_MISALIGNED, "out not 16-byte aligned");
+        a.out = static_cast<__half*>(v->out);
+    }
+    if (plan->n_prefix_pages + plan->n_suffix_pages) {
+        if (!v->q || !v->hot_k || !v->hot_v) return fail(WEAVER_ERR_INVALID_ARGUMENT, "q or the hot views are null");
+        if (!aligned16(v->q) || !aligned16(v->hot_k) || !aligned16(v->hot_v))
+            return fail(WEAVER_ERR_MISALIGNED, "q or the hot pool not 16-byte aligned");
+        if ((plan->n_prefix_pages && !v->prefix_refs) || (plan->n_suffix_pages && !v->suffix_refs))
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "block refs are null");
+        if (v->hot_pool_blocks == 0) return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_pool_blocks is 0");
+        if (v->hot_pool_blocks > (1ull << 27)) return fail(WEAVER_ERR_CAPACITY, "hot pool beyond 2^27 blocks");
+        for (const void* p : {static_cast<const void*>(v->prefix_refs), static_cast<const void*>(v->suffix_refs),
+                              static_cast<const void*>(v->prefix_lens), static_cast<const void*>(v->suffix_lens)})
+            if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(WEAVER_ERR_MISALIGNED, "block refs or lengths misaligned");
+    }
+    a.q = static_cast<const __half*>(v->q);
+    a.k = static_cast<const __half*>(v->hot_k);
+    a.v = static_cast<const __half*>(v->hot_v);
+    a.pool_blocks = v->hot_pool_blocks;
+    a.prefix_refs = v->prefix_refs;
+    a.suffix_refs = v->suffix_refs;
+    a.prefix_lens = v->prefix_lens;
+    a.suffix_lens = v->suffix_lens;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    plan->last_stream = s;
+    DeviceScope dev(plan->device);
+    WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
+    WEAVER_CUDA_TRY(launch_prefix(a, plan->n_items16, plan->merge, s), "prefix attention launch");
+    return WEAVER_OK;
+}
+
+int weaver_prefix_plan_status(weaver_prefix_plan* plan) {
+    if (!plan) return fail(WEAVER_ERR_INVALID_ARGUMENT, "null plan");
+    DeviceScope dev(plan->device);
+    WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
+    WEAVER_CUDA_TRY(cudaStreamSynchronize(plan->last_stream), "stream synchronize");
+    uint32_t st[2] = {0, 0};
+    WEAVER_CUDA_TRY(cudaMemcpy(st, plan->base.status, sizeof(st), cudaMemcpyDeviceToHost), "status read");
+    if (st[0] || st[1]) WEAVER_CUDA_TRY(cudaMemset(plan->base.status, 0, sizeof(st)), "status reset");
+    if (st[0] & DEVERR_TIMEOUT) return fail(WEAVER_ERR_TIMEOUT, "a device-side wait timed out (site %u)", st[1] & 0xFFu);
+    if (st[0] & DEVERR_REF_RANGE)
+        return fail(WEAVER_ERR_OUT_OF_RANGE, "a block reference was beyond the pool, or a length beyond its pages");
+    return WEAVER_OK;
+}
+
+}  // extern "C"

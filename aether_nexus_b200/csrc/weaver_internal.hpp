@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <vector>
+
 namespace weaver {
 
 constexpr uint32_t kBlock = 16;           // tokens per block (types.rs:159)
@@ -315,5 +317,84 @@ struct CombineArgs {
 };
 
 cudaError_t launch_combine(const CombineArgs& c, const float* packed, __half* out, cudaStream_t s);
+
+// ---- position rotation and the append into the hot pool (weaver_rope.cu) ----
+// Strides in elements (ts: token to token, hs: head to head); the D elements
+// of a head are contiguous.  freq: the pairs' frequencies as 64-bit
+// fixed-point fractions of a turn per position.
+struct RopeArgs {
+    const void *q, *k, *v;             // v only for the append (null: K only)
+    const void *q_weight, *k_weight;   // [D] of the inputs' type, or null: no norm
+    void *q_out, *k_out;               // k_out only for the rotation alone
+    void *hot_k, *hot_v;               // the append's pools, f16 [pool_rows][Hkv][D]
+    uint64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, qo_ts, qo_hs, ko_ts, ko_hs;
+    const int32_t* positions;
+    const int64_t* slots;
+    uint32_t* bad;
+    uint64_t pool_rows;
+    uint32_t T, Hq, Hkv, D, rot;
+    uint32_t bf16, interleaved;
+    uint32_t tokens_per_cta;           // set by the launcher
+    float eps, amplitude;
+    uint64_t freq[64];
+};
+cudaError_t launch_rope(RopeArgs a, bool append, cudaStream_t s);
+
+// ---- attention for a batch that shares prefixes (weaver_prefix.cu) ----
+// A page list: lists 0 .. n_groups-1 are the groups' prefixes, list n_groups +
+// b sequence b's own pages.
+struct PrefixList {
+    uint32_t tok0, ntok;       // its query tokens
+    uint32_t ref0, blocks;     // its pages in prefix_refs / suffix_refs
+    uint32_t tile0, n_tiles;   // first tile; row tiles per kv head
+    uint32_t tile_rows;        // rows of a tile
+    uint32_t causal;
+};
+// Rows row0 .. of one list's rows of one kv head.  Its items' partials are
+// n_slots runs of its rows from part_row0.
+struct PrefixTile {
+    uint64_t part_row0;
+    uint32_t list, kvh, row0;
+    uint32_t n_slots, direct;  // direct: its only item writes the output
+    uint32_t pad;
+};
+// Pages blk0 .. blk1-1 of a tile's list.
+struct PrefixItem {
+    uint64_t part_row;
+    uint32_t tile, blk0, blk1, pad;
+};
+struct PrefixArgs {
+    const __half *q, *k, *v;
+    __half* out;
+    float *out_m, *out_l, *out_o;      // partial outputs instead of out
+    const uint32_t *prefix_refs, *suffix_refs;
+    const uint32_t *prefix_lens, *suffix_lens;  // null: every page is full
+    uint64_t pool_blocks;
+    const PrefixItem* items;
+    const PrefixTile* tiles;
+    const PrefixList* lists;
+    const uint32_t *tok_seq, *seq_group;
+    float2* part_ml;
+    float* part_o;
+    uint32_t* status;
+    uint32_t n_groups, n_tokens, Hq, Hkv, G, D;
+    float scale;
+};
+// The host's view of a plan's geometry and the tables made from it.
+struct PrefixGeometry {
+    uint32_t n_groups, n_seqs, Hq, Hkv, D;
+    bool causal, partials;
+    const uint32_t *q_indptr, *group_indptr, *prefix_indptr, *suffix_indptr;
+};
+struct PrefixTables {
+    std::vector<PrefixList> lists;
+    std::vector<PrefixTile> tiles;
+    std::vector<PrefixItem> items16;
+    std::vector<uint32_t> tok_seq, seq_group;
+    uint64_t part_rows = 0;
+    bool needs_merge = false;
+};
+void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t);
+cudaError_t launch_prefix(const PrefixArgs& a, uint32_t n_items16, bool merge, cudaStream_t s);
 
 }  // namespace weaver

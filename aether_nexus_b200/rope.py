@@ -1,0 +1,252 @@
+"""Position rotation of query and key heads and the append into the paged hot
+pool (``weaver_rope_*``).
+
+The hot pool holds rotated keys.  :meth:`Rope.append` makes them where they are
+needed: in one kernel it rotates (and, with weights, first RMS-norms) the
+query and key heads of a batch of new tokens, writes K and V into the tokens'
+slots of the hot pool and q where the attention of the same stream reads it
+(``WeaverPlan.run``, ``PrefixPlan.run``).  :meth:`Rope.rotate` is the same
+without the pool, for keys that live in a flat cache
+(``WeaverEngine.multihead_attention``).
+
+A decode step of a batch::
+
+    rope = Rope(engine, head_dim=128, theta=500000.0)
+    slots = token_slots(refs, indptr, lens, q_indptr)          # host; or kept on the device
+    rope.append(q, k, v, positions, slots, hot_k, hot_v, q_out, bad_flag)
+    plan.run(q=q_out, hot_k=hot_k, hot_v=hot_v, ...)
+
+The reference's rotation is ``ops.metal:107-160``, its append to a flat cache
+``inference.rs:504-562``.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+
+from . import _native as N
+from .types import BLOCK_SIZE, REF_MASK
+from .weaver import _dptr, _stream_handle
+
+LAYOUTS = {"half": N.ROPE_HALF, "interleaved": N.ROPE_INTERLEAVED}
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[np.ndarray, float]:
+    """(radians per position of every pair, factor on cosines and sines) in
+    64 bits.  ``scaling`` stretches the rotation for contexts beyond the
+    trained one, ``{"type": ..., "factor": s, ...}``:
+
+    * ``linear``: every frequency / s;
+    * ``ntk``: theta * s^(r / (r - 2)), so the slowest pair is scaled by s and
+      the fastest not at all;
+    * ``yarn`` (Peng et al. 2023; ``original_length``, ``beta_fast`` = 32,
+      ``beta_slow`` = 1): pairs that turn more than beta_fast times over the
+      original length keep their frequency, those below beta_slow times take
+      f / s, a linear ramp over the pair index between; cosines and sines
+      times ``attention_factor`` (default 0.1 ln s + 1);
+    * ``bands`` (``original_length``, ``low`` = 1, ``high`` = 4): f / s where
+      the wavelength exceeds original_length / low, f where it is below
+      original_length / high, between them interpolated in the number of
+      turns."""
+    if rot_dim < 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim}")
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"theta {theta}")
+    i = np.arange(rot_dim // 2, dtype=np.float64)
+    f = float(theta) ** (-2.0 * i / max(rot_dim, 1))
+    if not scaling:
+        return f, 1.0
+    kind, s = scaling.get("type"), float(scaling["factor"])
+    known = {"linear": set(), "ntk": set(), "yarn": {"original_length", "beta_fast", "beta_slow", "attention_factor"},
+             "bands": {"original_length", "low", "high"}}
+    if kind not in known:
+        raise ValueError(f"unknown rope scaling {kind!r}")
+    extra = set(scaling) - known[kind] - {"type", "factor"}
+    if extra:
+        raise ValueError(f"rope scaling {kind!r} does not take {sorted(extra)}")
+    if not (math.isfinite(s) and s > 0):
+        raise ValueError(f"rope scaling factor {s}")
+    if kind == "linear":
+        return f / s, 1.0
+    if kind == "ntk":
+        if rot_dim <= 2:
+            raise ValueError("ntk scaling needs rot_dim > 2")
+        return (float(theta) * s ** (rot_dim / (rot_dim - 2.0))) ** (-2.0 * i / rot_dim), 1.0
+    length = float(scaling["original_length"])
+    turns = length * f / (2.0 * math.pi)  # of each pair over the original length
+    if kind == "yarn":
+        if theta == 1.0:
+            raise ValueError("yarn scaling needs theta != 1")
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+        def pair_of(n):  # the (fractional) pair that turns n times
+            return rot_dim * math.log(length / (n * 2.0 * math.pi)) / (2.0 * math.log(theta))
+        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim // 2 - 1)
+        ramp = np.clip((i - low) / max(high - low, 1e-3), 0.0, 1.0)
+        factor = scaling.get("attention_factor")
+        return f * (1.0 - ramp) + f / s * ramp, (0.1 * math.log(s) + 1.0) if factor is None else float(factor)
+    lo, hi = float(scaling.get("low", 1.0)), float(scaling.get("high", 4.0))
+    if hi <= lo:
+        raise ValueError("bands scaling needs high > low")
+    keep = np.clip((turns - lo) / (hi - lo), 0.0, 1.0)
+    return f * keep + f / s * (1.0 - keep), 1.0
+
+
+def token_slots(refs, indptr, lens, q_indptr) -> np.ndarray:
+    """Pool slots of the batch's new tokens (host arrays in, int64 out): the
+    queries ``q_indptr[b] .. q_indptr[b+1]`` of sequence b are the tokens that
+    follow its first ``lens[b]``, in the pages ``refs[indptr[b]:indptr[b+1]]``."""
+    refs = np.asarray(refs, np.uint32) & np.uint32(REF_MASK)
+    out = np.empty(int(q_indptr[-1]), np.int64)
+    for b in range(len(lens)):
+        n = int(q_indptr[b + 1]) - int(q_indptr[b])
+        idx = int(lens[b]) + np.arange(n, dtype=np.int64)
+        pages = refs[int(indptr[b]):int(indptr[b + 1])]
+        if n and int(idx[-1]) >= len(pages) * BLOCK_SIZE:
+            raise ValueError(f"sequence {b} needs {int(idx[-1]) // BLOCK_SIZE + 1} pages and has {len(pages)}")
+        out[int(q_indptr[b]):int(q_indptr[b + 1])] = pages[idx // BLOCK_SIZE].astype(np.int64) * BLOCK_SIZE + \
+            idx % BLOCK_SIZE
+    return out
+
+
+class Rope:
+    """The rotation of one head geometry (see :func:`rope_frequencies` for
+    ``theta`` and ``scaling``; ``inv_freq`` gives the frequencies directly).
+    ``layout`` pairs element i with i + rot_dim/2 (``"half"``) or 2i with 2i+1
+    (``"interleaved"``); elements from ``rot_dim`` on are not rotated."""
+
+    def __init__(self, engine, *, head_dim: int, rot_dim: int | None = None, theta: float = 10000.0,
+                 layout: str = "half", scaling: dict | None = None, inv_freq=None, amplitude: float | None = None):
+        rot_dim = head_dim if rot_dim is None else int(rot_dim)
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout {layout!r}, not one of {sorted(LAYOUTS)}")
+        if inv_freq is None:
+            f, amp = rope_frequencies(rot_dim, theta, scaling)
+        elif scaling is not None:
+            raise ValueError("inv_freq and scaling exclude each other")
+        else:
+            f, amp = np.asarray(inv_freq, np.float64), 1.0
+        f = np.ascontiguousarray(f, dtype=np.float64)
+        if f.shape != (rot_dim // 2,):
+            raise ValueError(f"inv_freq needs rot_dim / 2 = {rot_dim // 2} values")
+        self.inv_freq, self.amplitude = f, amp if amplitude is None else float(amplitude)
+        self.head_dim, self.rot_dim, self.layout, self.device = int(head_dim), rot_dim, layout, engine.device
+        c = N.RopeConfigC(self.head_dim, rot_dim, LAYOUTS[layout], self.amplitude, f.ctypes.data)
+        h = ctypes.c_void_p()
+        N.check(N.lib().weaver_rope_create(engine.handle, ctypes.byref(c), ctypes.byref(h)))
+        self._h = h
+
+    def _stream(self, stream):
+        if stream is None:  # the current stream of the object's device, which need not be the current one
+            import torch
+            stream = torch.cuda.current_stream(self.device)
+        return _stream_handle(stream)
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            N.lib().weaver_rope_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _check(self, name, t, shape, dtype):
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{name} must be a CUDA tensor on device {self.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+        return t
+
+    def _views(self, q, k, positions, q_weight, k_weight, eps) -> N.RopeViewsC:
+        import torch
+        if q is None and k is None:
+            raise ValueError("neither q nor k given")
+        lead = q if q is not None else k
+        if lead.dim() != 3:
+            raise ValueError("heads are [tokens, heads, head_dim] tensors")
+        T, dt = int(lead.shape[0]), lead.dtype
+        if dt not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"heads are {dt}, not float16 or bfloat16")
+        v = N.RopeViewsC()
+        v.n_tokens, v.dtype, v.eps = T, N.F16 if dt == torch.float16 else N.BF16, float(eps)
+        if q is not None:
+            self._check("q", q, (T, q.shape[1], self.head_dim), dt)
+            v.q, v.q_heads, v.q_token_stride, v.q_head_stride = q.data_ptr(), q.shape[1], q.stride(0), q.stride(1)
+        if k is not None:
+            self._check("k", k, (T, k.shape[1], self.head_dim), dt)
+            v.k, v.kv_heads, v.k_token_stride, v.k_head_stride = k.data_ptr(), k.shape[1], k.stride(0), k.stride(1)
+        self._check("positions", positions, (T,), torch.int32)
+        v.positions = positions.data_ptr()
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None:
+                setattr(v, name, self._check(name, w, (self.head_dim,), dt).data_ptr())
+        return v
+
+    def rotate(self, q, k, positions, q_out, k_out=None, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+               stream=None) -> None:
+        """``q_out`` / ``k_out`` = the rotated (with a weight: normed, then
+        rotated) ``q [T, Hq, d]`` / ``k [T, Hkv, d]`` (float16 or bfloat16, any
+        token and head strides; outputs of the inputs' type, the input itself
+        included).  ``q`` or ``k`` may be None.  ``positions [T]`` int32."""
+        v = self._views(q, k, positions, q_weight, k_weight, eps)
+        if q is not None:
+            self._check("q_out", q_out, q.shape, q.dtype)
+            v.q_out, v.q_out_token_stride, v.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+        if k is not None:
+            self._check("k_out", k_out, k.shape, k.dtype)
+            v.k_out, v.k_out_token_stride, v.k_out_head_stride = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+        N.check(N.lib().weaver_rope_rotate(self._h, ctypes.byref(v), self._stream(stream)))
+
+    def append(self, q, k, v, positions, slots, hot_k, hot_v, q_out, bad_flag, *, q_weight=None, k_weight=None,
+               eps: float = 1e-6, hot_pool_blocks: int | None = None, stream=None) -> None:
+        """Rotates ``q [T, Hq, d]`` into ``q_out`` (float16) and ``k [T, Hkv,
+        d]`` into row ``slots[t]`` (int64: block * 16 + row; negative: padding,
+        skipped) of ``hot_k [blocks, 16, Hkv, d]``, and copies ``v`` into
+        ``hot_v``.  ``q`` (with ``q_out``) and ``v`` (with ``hot_v``) may be
+        None.  ``hot_k`` / ``hot_v`` may be raw device pointers (a
+        ``DeviceFabric`` layer's) with ``hot_pool_blocks``.  ``bad_flag`` (one
+        int32) gets 1 OR-ed in for a slot beyond the pool, whose token is
+        skipped.  The slots of one call must be distinct."""
+        import torch
+        if k is None:
+            raise ValueError("append needs k")
+        x = self._views(q, k, positions, q_weight, k_weight, eps)
+        T, hkv = int(k.shape[0]), int(k.shape[1])
+        if q is not None:
+            self._check("q_out", q_out, q.shape, torch.float16)
+            x.q_out, x.q_out_token_stride, x.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+        if (v is None) != (hot_v is None):
+            raise ValueError("v and hot_v come together")
+        if v is not None:
+            self._check("v", v, k.shape, k.dtype)
+            x.v, x.v_token_stride, x.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
+        blocks = hot_pool_blocks
+        for name, pool in (("hot_k", hot_k), ("hot_v", hot_v)):
+            if pool is None or isinstance(pool, int):
+                continue
+            self._check(name, pool, (pool.shape[0], BLOCK_SIZE, hkv, self.head_dim), torch.float16)
+            if not pool.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if blocks is None:
+                blocks = int(pool.shape[0])
+            if int(pool.shape[0]) < blocks:
+                raise ValueError(f"{name} has fewer than {blocks} blocks")
+        if blocks is None:
+            raise ValueError("raw pool pointers need hot_pool_blocks")
+        self._check("slots", slots, (T,), torch.int64)
+        self._check("bad_flag", bad_flag.reshape(-1)[:1], (1,), torch.int32)
+        x.slots, x.bad_flag = slots.data_ptr(), bad_flag.data_ptr()
+        x.hot_k, x.hot_v, x.hot_pool_blocks = _dptr(hot_k), _dptr(hot_v), blocks
+        N.check(N.lib().weaver_rope_append(self._h, ctypes.byref(x), self._stream(stream)))
+
+
+__all__ = ["Rope", "rope_frequencies", "token_slots"]

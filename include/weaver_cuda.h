@@ -455,6 +455,136 @@ WEAVER_EXPORT int weaver_migrate_blocks(const void* hot_k, const void* hot_v, ui
                                         weaver_sparse_code* cold_v, uint64_t cold_pool_blocks, uint32_t* bad_flag,
                                         void* stream);
 
+/* ---- position rotation and the append into the hot pool --------------------
+ * The keys of the hot pool are rotated keys; these two calls make them on the
+ * device, next to the step that reads them.  The reference rotates and
+ * appends to a flat cache in its full loop (ops.metal:107-160,
+ * inference.rs:504-562) and fills the hot pool from the host only.
+ *
+ * weaver_rope holds a head's rotation: pair i of the first rot_dim elements
+ * turns by position * inv_freq[i]; HALF pairs (i, i + rot_dim/2), INTERLEAVED
+ * pairs (2i, 2i + 1); elements from rot_dim on pass through.  Angles are
+ * exact to about 2^-26 of a turn at any position (64-bit fixed point).  With
+ * a weight each head x is first replaced by x * rsqrt(mean(x^2) + eps) *
+ * weight.  Arithmetic in fp32, rounded once to the output's type.  The object
+ * holds no device memory and may be used by several threads and captured
+ * graphs at once. */
+enum weaver_dtype { WEAVER_F16 = 0, WEAVER_BF16 = 1 };
+enum weaver_rope_layout { WEAVER_ROPE_HALF = 0, WEAVER_ROPE_INTERLEAVED = 1 };
+
+typedef struct weaver_rope_config {
+    uint32_t head_dim;      /* 64 or 128 */
+    uint32_t rot_dim;       /* a multiple of 16, 0 .. head_dim (0: norm only) */
+    uint32_t layout;        /* weaver_rope_layout */
+    float amplitude;        /* factor on every cosine and sine (1 without scaling) */
+    const double* inv_freq; /* host, rot_dim / 2 values: radians per position */
+} weaver_rope_config;
+
+/* Strides are in elements, multiples of 8; a head's head_dim elements are
+ * contiguous.  All pointers 16-byte aligned device pointers. */
+typedef struct weaver_rope_views {
+    uint32_t n_tokens, q_heads, kv_heads;
+    uint32_t dtype;            /* weaver_dtype of q, k, v and the weights */
+    const void* q;             /* [n_tokens][q_heads][head_dim]; null with q_heads = 0 */
+    const void* k;             /* [n_tokens][kv_heads][head_dim]; null with kv_heads = 0 */
+    const void* v;             /* append only; null with hot_v (the pool's one region for K and V) */
+    uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int32_t* positions;  /* [n_tokens], negative ones included */
+    const void* q_weight;      /* [head_dim], or null: no norm of the query heads */
+    const void* k_weight;      /* [head_dim], or null: no norm of the key heads */
+    float eps;
+    uint32_t _pad;
+    void* q_out;               /* rotate: q's type; append: f16.  May be q itself (same strides) */
+    void* k_out;               /* rotate only.  May be k itself (same strides) */
+    uint64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+    /* append only */
+    const int64_t* slots;      /* [n_tokens]: block * 16 + row in the hot pool, negative: a padding token */
+    void* hot_k;               /* f16 [hot_pool_blocks][16][kv_heads][head_dim] */
+    void* hot_v;
+    uint64_t hot_pool_blocks;
+    uint32_t* bad_flag;        /* device word; 1 is OR-ed in for a slot beyond the pool */
+} weaver_rope_views;
+
+typedef struct weaver_rope weaver_rope;
+WEAVER_EXPORT int weaver_rope_create(weaver_engine* engine, const weaver_rope_config* config, weaver_rope** out);
+WEAVER_EXPORT void weaver_rope_destroy(weaver_rope* rope);
+/* q_out / k_out = the rotated (normed) q / k.  One kernel. */
+WEAVER_EXPORT int weaver_rope_rotate(weaver_rope* rope, const weaver_rope_views* views, void* stream);
+/* The same, with k and v going to row slots[t] of the hot pool (K rotated, V
+ * as it is) and q to q_out, ready for weaver_run or weaver_prefix_run on the
+ * same stream.  A token with a negative slot (the padding behind the last
+ * sequence) or one beyond the pool is skipped: neither the pool nor its row of
+ * q_out is written.  The slots of one call are distinct: of two tokens with
+ * the same slot either may win, separately for every head.  bf16 values
+ * beyond f16's range become infinite.  One kernel, CUDA-graph capturable. */
+WEAVER_EXPORT int weaver_rope_append(weaver_rope* rope, const weaver_rope_views* views, void* stream);
+
+/* ---- attention for a batch that shares prefixes ------------------------------
+ * Exact attention over the hot pool in token lengths.  num_seqs sequences in
+ * num_groups groups of neighbours; sequence b has queries q_indptr[b] ..
+ * q_indptr[b+1]-1 and pages suffix_indptr[b] .. of suffix_refs of its own,
+ * and its group's pages prefix_indptr[g] .. of prefix_refs, which are read
+ * once for all queries of the group.  With nq queries of its own, query j of
+ * a sequence attends to the whole prefix and, with WEAVER_FLAG_CAUSAL, to the
+ * first suffix_len - nq + 1 + j tokens of its own pages (none where that is
+ * not positive; the rule of ops.metal:549), else to all of them; scale * q.K,
+ * one softmax over both.  A query that sees nothing gives zeros.
+ * One token per sequence, draft batches and prompt chunks may be mixed; a
+ * group of one sequence with no prefix is a plain paged sequence.
+ *
+ * The tokens of the last page past a length, and pages past it, are not part
+ * of the result whatever the pool holds there.  A NaN or infinite value at a
+ * position that some query of a call sees can turn the outputs of other
+ * queries of that head NaN too, causally masked or not.
+ * WEAVER_FLAG_PARTIALS writes (m, l, o) instead of out, as weaver_run does, so
+ * that a plan over cold blocks of the same queries can be merged with
+ * weaver_merge_partials. */
+typedef struct weaver_prefix_shape {
+    uint32_t num_groups, num_seqs;
+    uint32_t q_heads, kv_heads, head_dim; /* q_heads % kv_heads == 0; head_dim 64 or 128 */
+    float scale;
+    uint32_t flags;                       /* WEAVER_FLAG_CAUSAL, WEAVER_FLAG_PARTIALS */
+    uint32_t _pad;
+} weaver_prefix_shape;
+
+typedef struct weaver_prefix_views {
+    const void* q;                /* f16 [q_indptr[num_seqs]][q_heads][head_dim] */
+    const void* hot_k;            /* f16 [hot_pool_blocks][16][kv_heads][head_dim] */
+    const void* hot_v;            /* same layout (may equal hot_k) */
+    uint64_t hot_pool_blocks;
+    const uint32_t* prefix_refs;  /* block refs (bit 31 ignored) */
+    const uint32_t* suffix_refs;
+    const uint32_t* prefix_lens;  /* device, [num_groups] tokens; null: every page is full */
+    const uint32_t* suffix_lens;  /* device, [num_seqs] tokens; null: every page is full */
+    void* out;                    /* f16, q's shape */
+    float* part_m;                /* WEAVER_FLAG_PARTIALS: [tokens][q_heads] */
+    float* part_l;
+    float* part_o;                /* [tokens][q_heads][head_dim] */
+} weaver_prefix_views;
+
+typedef struct weaver_prefix_plan weaver_prefix_plan;
+/* Host arrays: group_indptr [num_groups + 1] (sequences), prefix_indptr
+ * [num_groups + 1] (pages), q_indptr [num_seqs + 1] (queries), suffix_indptr
+ * [num_seqs + 1] (pages).  The page counts are capacities: the lengths may
+ * change from run to run on the device, up to 16 tokens per page, so one plan
+ * (and one captured graph) serves a sequence until it needs a page more. */
+WEAVER_EXPORT int weaver_prefix_plan_create(weaver_engine* engine, const weaver_prefix_shape* shape,
+                                            const uint32_t* q_indptr, const uint32_t* group_indptr,
+                                            const uint32_t* prefix_indptr, const uint32_t* suffix_indptr,
+                                            weaver_prefix_plan** out);
+WEAVER_EXPORT void weaver_prefix_plan_destroy(weaver_prefix_plan* plan);
+/* Launches the attention on `stream`: no allocation, no host synchronisation,
+ * CUDA-graph capturable.  Only one run of a plan may be in flight at a time,
+ * replayed graphs included (the plan owns the partials). */
+WEAVER_EXPORT int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* views, void* stream);
+/* Number of kernels one weaver_prefix_run launches. */
+WEAVER_EXPORT int weaver_prefix_plan_kernel_count(const weaver_prefix_plan* plan);
+/* Synchronises the plan's last stream, then reads and clears its status:
+ * WEAVER_OK, WEAVER_ERR_OUT_OF_RANGE (a block ref beyond the pool, whose
+ * tokens were skipped, or a length beyond its pages, which was cut) or
+ * WEAVER_ERR_TIMEOUT. */
+WEAVER_EXPORT int weaver_prefix_plan_status(weaver_prefix_plan* plan);
+
 /* ---- self-test of the bounded device-side waits --------------------------
  * No counterpart in the reference (its kernel has no waits and no error
  * path).  Every wait in this library's kernels gives up after a time limit,

@@ -30,6 +30,11 @@ pub const WEAVER_FLAG_CAUSAL: u32 = 1;
 pub const WEAVER_FLAG_QLATENT_INPUT: u32 = 2;
 pub const WEAVER_FLAG_PARTIALS: u32 = 4;
 
+pub const WEAVER_F16: u32 = 0;
+pub const WEAVER_BF16: u32 = 1;
+pub const WEAVER_ROPE_HALF: u32 = 0;
+pub const WEAVER_ROPE_INTERLEAVED: u32 = 1;
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default, PartialEq, Eq)]
 pub struct weaver_sparse_code {
@@ -189,6 +194,91 @@ pub struct weaver_combine {
     _private: [u8; 0],
 }
 
+/// Opaque position rotation of one head geometry.
+#[repr(C)]
+pub struct weaver_rope {
+    _private: [u8; 0],
+}
+/// Opaque plan of the attention for a batch that shares prefixes.
+#[repr(C)]
+pub struct weaver_prefix_plan {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct weaver_rope_config {
+    pub head_dim: u32,
+    pub rot_dim: u32,
+    pub layout: u32,
+    pub amplitude: f32,
+    pub inv_freq: *const f64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct weaver_rope_views {
+    pub n_tokens: u32,
+    pub q_heads: u32,
+    pub kv_heads: u32,
+    pub dtype: u32,
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub q_token_stride: u64,
+    pub q_head_stride: u64,
+    pub k_token_stride: u64,
+    pub k_head_stride: u64,
+    pub v_token_stride: u64,
+    pub v_head_stride: u64,
+    pub positions: *const i32,
+    pub q_weight: *const c_void,
+    pub k_weight: *const c_void,
+    pub eps: f32,
+    pub _pad: u32,
+    pub q_out: *mut c_void,
+    pub k_out: *mut c_void,
+    pub q_out_token_stride: u64,
+    pub q_out_head_stride: u64,
+    pub k_out_token_stride: u64,
+    pub k_out_head_stride: u64,
+    pub slots: *const i64,
+    pub hot_k: *mut c_void,
+    pub hot_v: *mut c_void,
+    pub hot_pool_blocks: u64,
+    pub bad_flag: *mut u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct weaver_prefix_shape {
+    pub num_groups: u32,
+    pub num_seqs: u32,
+    pub q_heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub scale: f32,
+    pub flags: u32,
+    pub _pad: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct weaver_prefix_views {
+    pub q: *const c_void,
+    pub hot_k: *const c_void,
+    pub hot_v: *const c_void,
+    pub hot_pool_blocks: u64,
+    pub prefix_refs: *const u32,
+    pub suffix_refs: *const u32,
+    pub prefix_lens: *const u32,
+    pub suffix_lens: *const u32,
+    pub out: *mut c_void,
+    pub part_m: *mut f32,
+    pub part_l: *mut f32,
+    pub part_o: *mut f32,
+}
+
 extern "C" {
     pub fn weaver_abi_version() -> c_int;
     pub fn weaver_last_error() -> *const c_char;
@@ -275,6 +365,21 @@ extern "C" {
     pub fn weaver_distill_stats(rows: *const c_void, n_rows: u32, kv_heads: u32, head_dim: u32,
                                 dictionary: *const c_void, dict_size: u32, dict_head_stride: u64,
                                 out_codes: *mut weaver_sparse_code, diag: *mut u32, stream: *mut c_void) -> c_int;
+
+    pub fn weaver_rope_create(engine: *mut weaver_engine, config: *const weaver_rope_config,
+                              out: *mut *mut weaver_rope) -> c_int;
+    pub fn weaver_rope_destroy(rope: *mut weaver_rope);
+    pub fn weaver_rope_rotate(rope: *mut weaver_rope, views: *const weaver_rope_views, stream: *mut c_void) -> c_int;
+    pub fn weaver_rope_append(rope: *mut weaver_rope, views: *const weaver_rope_views, stream: *mut c_void) -> c_int;
+
+    pub fn weaver_prefix_plan_create(engine: *mut weaver_engine, shape: *const weaver_prefix_shape,
+                                     q_indptr: *const u32, group_indptr: *const u32, prefix_indptr: *const u32,
+                                     suffix_indptr: *const u32, out: *mut *mut weaver_prefix_plan) -> c_int;
+    pub fn weaver_prefix_plan_destroy(plan: *mut weaver_prefix_plan);
+    pub fn weaver_prefix_run(plan: *mut weaver_prefix_plan, views: *const weaver_prefix_views,
+                             stream: *mut c_void) -> c_int;
+    pub fn weaver_prefix_plan_kernel_count(plan: *const weaver_prefix_plan) -> c_int;
+    pub fn weaver_prefix_plan_status(plan: *mut weaver_prefix_plan) -> c_int;
 }
 
 #[cfg(test)]
@@ -292,5 +397,9 @@ mod tests {
         assert_eq!(size_of::<weaver_shape>(), 32);
         assert_eq!(size_of::<weaver_views>(), 17 * 8);
         assert_eq!(align_of::<weaver_views>(), 8);
+        assert_eq!(size_of::<weaver_rope_config>(), 24);
+        assert_eq!(size_of::<weaver_rope_views>(), 208);
+        assert_eq!(size_of::<weaver_prefix_shape>(), 32);
+        assert_eq!(size_of::<weaver_prefix_views>(), 96);
     }
 }
