@@ -1847,6 +1847,23 @@ struct weaver_rope {
 
 namespace {
 
+// A hot pool as [blocks * 2][Hkv * D / 64][8 rows][64] f16: a box of one head's
+// part of one page, 128-byte swizzle.  Read past the pool's end it is zero.
+int encode_pages(CUtensorMap* map, const void* base, uint64_t blocks, uint64_t Hkv, uint64_t D, const char* what) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(WEAVER_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t row = Hkv * D * 2;
+    cuuint64_t dims[4] = {64, 8, Hkv * D / 64, blocks * 2};
+    cuuint64_t strides[3] = {row, 128, 8 * row};
+    cuuint32_t box[4] = {64, 8, static_cast<cuuint32_t>(D / 64), 2};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(WEAVER_ERR_CUDA, "tensor map for %s failed (CUresult %d)", what, (int)r);
+    return WEAVER_OK;
+}
+
 // Makes `device` current for one call and puts the caller's device back.
 struct DeviceScope {
     int before = -1;
@@ -1958,7 +1975,7 @@ struct weaver_prefix_plan {
     weaver_prefix_shape shape{};
     PrefixArgs base{};
     void* arena = nullptr;
-    uint32_t n_items16 = 0;
+    uint32_t n_items16 = 0, n_tc_ctas = 0;
     bool merge = false;
     uint64_t n_prefix_pages = 0, n_suffix_pages = 0;
     cudaStream_t last_stream = nullptr;
@@ -2045,7 +2062,8 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
                        q_indptr, group_indptr, prefix_indptr, suffix_indptr};
     PrefixTables t;
     plan_prefix(geo, static_cast<uint32_t>(eng->prop.multiProcessorCount), &t);
-    if (t.items16.size() > 0x7FFFFFFFull || t.tiles.size() > 0x7FFFFFFFull) return fail(WEAVER_ERR_CAPACITY, "too many work items");
+    if (t.items16.size() > 0x7FFFFFFFull || t.items_tc.size() > 0x7FFFFFFFull)
+        return fail(WEAVER_ERR_CAPACITY, "too many work items");
 
     // one allocation: tables, status, partials
     size_t off = 0;
@@ -2055,9 +2073,10 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
         return o;
     };
     const size_t o_lists = place(t.lists.size() * sizeof(PrefixList)), o_tiles = place(t.tiles.size() * sizeof(PrefixTile)),
-                 o_items = place(t.items16.size() * sizeof(PrefixItem)), o_seq = place(t.tok_seq.size() * 4),
-                 o_group = place(t.seq_group.size() * 4), o_status = place(8), o_ml = place(t.part_rows * sizeof(float2)),
-                 o_o = place(t.part_rows * D * sizeof(float));
+                 o_items = place(t.items16.size() * sizeof(PrefixItem)), o_tc = place(t.items_tc.size() * sizeof(PrefixItem)),
+                 o_ptr = place(t.tc_ptr.size() * 4), o_row = place(t.row_tok.size() * 4),
+                 o_tok = place(t.tok_lists.size() * sizeof(uint4)), o_status = place(8),
+                 o_ml = place(t.part_rows * sizeof(float2)), o_o = place(t.part_rows * D * sizeof(float));
     auto plan = std::unique_ptr<weaver_prefix_plan>(new weaver_prefix_plan());
     plan->device = eng->device;
     cudaError_t e = cudaMalloc(&plan->arena, off);
@@ -2069,8 +2088,10 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     upload(o_lists, t.lists.data(), t.lists.size() * sizeof(PrefixList));
     upload(o_tiles, t.tiles.data(), t.tiles.size() * sizeof(PrefixTile));
     upload(o_items, t.items16.data(), t.items16.size() * sizeof(PrefixItem));
-    upload(o_seq, t.tok_seq.data(), t.tok_seq.size() * 4);
-    upload(o_group, t.seq_group.data(), t.seq_group.size() * 4);
+    upload(o_tc, t.items_tc.data(), t.items_tc.size() * sizeof(PrefixItem));
+    upload(o_ptr, t.tc_ptr.data(), t.tc_ptr.size() * 4);
+    upload(o_row, t.row_tok.data(), t.row_tok.size() * 4);
+    upload(o_tok, t.tok_lists.data(), t.tok_lists.size() * sizeof(uint4));
     const uint32_t zero[2] = {0, 0};
     upload(o_status, zero, sizeof(zero));
     if (e != cudaSuccess) {
@@ -2079,6 +2100,7 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     }
     plan->shape = *sh;
     plan->n_items16 = static_cast<uint32_t>(t.items16.size());
+    plan->n_tc_ctas = static_cast<uint32_t>(t.tc_ptr.size()) - 1;
     plan->merge = t.needs_merge;
     plan->n_prefix_pages = prefix_indptr[NG];
     plan->n_suffix_pages = suffix_indptr[B];
@@ -2086,12 +2108,13 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     a.lists = reinterpret_cast<const PrefixList*>(base + o_lists);
     a.tiles = reinterpret_cast<const PrefixTile*>(base + o_tiles);
     a.items = reinterpret_cast<const PrefixItem*>(base + o_items);
-    a.tok_seq = reinterpret_cast<const uint32_t*>(base + o_seq);
-    a.seq_group = reinterpret_cast<const uint32_t*>(base + o_group);
+    a.tc_items = reinterpret_cast<const PrefixItem*>(base + o_tc);
+    a.tc_ptr = reinterpret_cast<const uint32_t*>(base + o_ptr);
+    a.row_tok = reinterpret_cast<const uint32_t*>(base + o_row);
+    a.tok_lists = reinterpret_cast<const uint4*>(base + o_tok);
     a.status = reinterpret_cast<uint32_t*>(base + o_status);
     a.part_ml = reinterpret_cast<float2*>(base + o_ml);
     a.part_o = reinterpret_cast<float*>(base + o_o);
-    a.n_groups = NG;
     a.n_tokens = q_indptr[B];
     a.Hq = Hq;
     a.Hkv = Hkv;
@@ -2113,7 +2136,7 @@ void weaver_prefix_plan_destroy(weaver_prefix_plan* plan) {
 
 int weaver_prefix_plan_kernel_count(const weaver_prefix_plan* plan) {
     if (!plan) return 0;
-    return (plan->n_items16 ? 1 : 0) + (plan->merge ? 1 : 0);
+    return (plan->n_tc_ctas ? 1 : 0) + (plan->n_items16 ? 1 : 0) + (plan->merge ? 1 : 0);
 }
 
 int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, void* stream) {
@@ -2157,7 +2180,15 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
     plan->last_stream = s;
     DeviceScope dev(plan->device);
     WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
-    WEAVER_CUDA_TRY(launch_prefix(a, plan->n_items16, plan->merge, s), "prefix attention launch");
+    if (plan->n_tc_ctas) {
+        CUtensorMap tm_k, tm_v;
+        int rc;
+        if ((rc = encode_pages(&tm_k, v->hot_k, v->hot_pool_blocks, a.Hkv, a.D, "hot_k"))) return rc;
+        if ((rc = encode_pages(&tm_v, v->hot_v, v->hot_pool_blocks, a.Hkv, a.D, "hot_v"))) return rc;
+        WEAVER_CUDA_TRY(launch_prefix_tc(a, tm_k, tm_v, plan->n_tc_ctas, s), "prefix attention launch");
+    }
+    if (plan->n_items16) WEAVER_CUDA_TRY(launch_prefix_rows16(a, plan->n_items16, s), "prefix attention launch");
+    if (plan->merge) WEAVER_CUDA_TRY(launch_prefix_merge(a, s), "prefix merge launch");
     return WEAVER_OK;
 }
 

@@ -340,28 +340,32 @@ struct RopeArgs {
 };
 cudaError_t launch_rope(RopeArgs a, bool append, cudaStream_t s);
 
-// ---- attention for a batch that shares prefixes (weaver_prefix.cu) ----
-// A page list: lists 0 .. n_groups-1 are the groups' prefixes, list n_groups +
-// b sequence b's own pages.
+// ---- attention for a batch that shares prefixes (weaver_prefix.cu, weaver_prefix_tc.cu) ----
+// A set of query tokens and the pages they attend to: a group's prefix pages,
+// then one sequence's own pages (either may be absent).  Row r of kv head g is
+// token row_tok[tok0 + r / G], q head g * G + r % G.
 struct PrefixList {
-    uint32_t tok0, ntok;       // its query tokens
-    uint32_t ref0, blocks;     // its pages in prefix_refs / suffix_refs
-    uint32_t tile0, n_tiles;   // first tile; row tiles per kv head
-    uint32_t tile_rows;        // rows of a tile
-    uint32_t causal;
+    uint32_t tok0, ntok;                     // its query tokens in row_tok
+    uint32_t pre_ref0, pre_blocks, pre_len;  // pages in prefix_refs; index into prefix_lens
+    uint32_t suf_ref0, suf_blocks, suf_len;  // pages in suffix_refs; index into suffix_lens
+    uint32_t tile0, n_tiles, tile_rows;      // first tile; row tiles per kv head; rows of a tile
+    uint32_t causal;                         // of the own pages
 };
-// Rows row0 .. of one list's rows of one kv head.  Its items' partials are
-// n_slots runs of its rows from part_row0.
+// Rows row0 .. of one list's rows of one kv head.  Its partials are n_slots
+// runs of its rows from part_row0.
 struct PrefixTile {
     uint64_t part_row0;
     uint32_t list, kvh, row0;
     uint32_t n_slots, direct;  // direct: its only item writes the output
     uint32_t pad;
 };
-// Pages blk0 .. blk1-1 of a tile's list.
+// Pages blk0 .. blk1-1 of a tile's list (16-row tiles), or 128-token tiles of
+// pages blk0 .. blk1-1 (tensor-memory tiles), counted over the prefix's pages
+// and then the own ones.
 struct PrefixItem {
     uint64_t part_row;
-    uint32_t tile, blk0, blk1, pad;
+    uint32_t tile, blk0, blk1;
+    uint32_t two;  // tensor-memory tiles of at most 128 rows: the two halves of the CTA write a slot each
 };
 struct PrefixArgs {
     const __half *q, *k, *v;
@@ -370,14 +374,17 @@ struct PrefixArgs {
     const uint32_t *prefix_refs, *suffix_refs;
     const uint32_t *prefix_lens, *suffix_lens;  // null: every page is full
     uint64_t pool_blocks;
-    const PrefixItem* items;
+    const PrefixItem* items;           // of the 16-row tiles
+    const PrefixItem* tc_items;        // of the tensor-memory tiles, CTA c's are [tc_ptr[c], tc_ptr[c+1])
+    const uint32_t* tc_ptr;
     const PrefixTile* tiles;
     const PrefixList* lists;
-    const uint32_t *tok_seq, *seq_group;
+    const uint32_t* row_tok;
+    const uint4* tok_lists;            // [tokens] (list, token of it) of its prefix part, of its own part; ~0: none
     float2* part_ml;
     float* part_o;
     uint32_t* status;
-    uint32_t n_groups, n_tokens, Hq, Hkv, G, D;
+    uint32_t n_tokens, Hq, Hkv, G, D;
     float scale;
 };
 // The host's view of a plan's geometry and the tables made from it.
@@ -389,12 +396,18 @@ struct PrefixGeometry {
 struct PrefixTables {
     std::vector<PrefixList> lists;
     std::vector<PrefixTile> tiles;
-    std::vector<PrefixItem> items16;
-    std::vector<uint32_t> tok_seq, seq_group;
+    std::vector<PrefixItem> items16, items_tc;
+    std::vector<uint32_t> tc_ptr, row_tok;
+    std::vector<uint4> tok_lists;
     uint64_t part_rows = 0;
     bool needs_merge = false;
 };
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t);
-cudaError_t launch_prefix(const PrefixArgs& a, uint32_t n_items16, bool merge, cudaStream_t s);
+cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s);
+cudaError_t launch_prefix_merge(const PrefixArgs& a, cudaStream_t s);
+// Tiles of up to 256 rows on tcgen05 (tm_k / tm_v: the pools as [blocks * 2][8
+// rows][Hkv * D / 64][64], boxes of one page of one head, 128-byte swizzle).
+cudaError_t launch_prefix_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas,
+                             cudaStream_t s);
 
 }  // namespace weaver
