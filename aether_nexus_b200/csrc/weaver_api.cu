@@ -1976,7 +1976,6 @@ struct weaver_prefix_plan {
     PrefixArgs base{};
     void* arena = nullptr;
     uint32_t n_items16 = 0, n_tc_ctas = 0;
-    bool merge = false;
     uint64_t n_prefix_pages = 0, n_suffix_pages = 0;
     cudaStream_t last_stream = nullptr;
 };
@@ -2065,35 +2064,29 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     if (t.items16.size() > 0x7FFFFFFFull || t.items_tc.size() > 0x7FFFFFFFull)
         return fail(WEAVER_ERR_CAPACITY, "too many work items");
 
-    // one allocation: tables, status, partials
-    size_t off = 0;
-    auto place = [&](size_t bytes) {
-        const size_t o = off;
-        off = align_up(off + bytes, 256);
+    // one allocation: the tables (one upload), the status, the partials
+    std::vector<char> image;
+    auto place = [&](const void* src, size_t bytes) {
+        const size_t o = align_up(image.size(), 256);
+        image.resize(o + bytes);
+        if (bytes) memcpy(image.data() + o, src, bytes);
         return o;
     };
-    const size_t o_lists = place(t.lists.size() * sizeof(PrefixList)), o_tiles = place(t.tiles.size() * sizeof(PrefixTile)),
-                 o_items = place(t.items16.size() * sizeof(PrefixItem)), o_tc = place(t.items_tc.size() * sizeof(PrefixItem)),
-                 o_ptr = place(t.tc_ptr.size() * 4), o_row = place(t.row_tok.size() * 4),
-                 o_tok = place(t.tok_lists.size() * sizeof(uint4)), o_status = place(8),
-                 o_ml = place(t.part_rows * sizeof(float2)), o_o = place(t.part_rows * D * sizeof(float));
+    const uint32_t zero[2] = {0, 0};
+    const size_t o_lists = place(t.lists.data(), t.lists.size() * sizeof(PrefixList)),
+                 o_tiles = place(t.tiles.data(), t.tiles.size() * sizeof(PrefixTile)),
+                 o_items = place(t.items16.data(), t.items16.size() * sizeof(PrefixItem)),
+                 o_tc = place(t.items_tc.data(), t.items_tc.size() * sizeof(PrefixTcItem)),
+                 o_ptr = place(t.tc_ptr.data(), t.tc_ptr.size() * 4), o_row = place(t.row_tok.data(), t.row_tok.size() * 4),
+                 o_merge = place(t.merge_rows.data(), t.merge_rows.size() * sizeof(PrefixMergeRow)),
+                 o_status = place(zero, sizeof(zero));
+    const size_t o_ml = align_up(image.size(), 256), o_o = align_up(o_ml + t.part_rows * sizeof(float2), 256);
     auto plan = std::unique_ptr<weaver_prefix_plan>(new weaver_prefix_plan());
     plan->device = eng->device;
-    cudaError_t e = cudaMalloc(&plan->arena, off);
+    cudaError_t e = cudaMalloc(&plan->arena, o_o + t.part_rows * D * sizeof(float) + 16);
     if (e != cudaSuccess) return cuda_fail(e, "prefix plan allocation");
     char* base = static_cast<char*>(plan->arena);
-    auto upload = [&](size_t o, const void* src, size_t bytes) {
-        if (e == cudaSuccess && bytes) e = cudaMemcpy(base + o, src, bytes, cudaMemcpyHostToDevice);
-    };
-    upload(o_lists, t.lists.data(), t.lists.size() * sizeof(PrefixList));
-    upload(o_tiles, t.tiles.data(), t.tiles.size() * sizeof(PrefixTile));
-    upload(o_items, t.items16.data(), t.items16.size() * sizeof(PrefixItem));
-    upload(o_tc, t.items_tc.data(), t.items_tc.size() * sizeof(PrefixItem));
-    upload(o_ptr, t.tc_ptr.data(), t.tc_ptr.size() * 4);
-    upload(o_row, t.row_tok.data(), t.row_tok.size() * 4);
-    upload(o_tok, t.tok_lists.data(), t.tok_lists.size() * sizeof(uint4));
-    const uint32_t zero[2] = {0, 0};
-    upload(o_status, zero, sizeof(zero));
+    e = cudaMemcpy(base, image.data(), image.size(), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
         cudaFree(plan->arena);
         return cuda_fail(e, "prefix plan upload");
@@ -2101,17 +2094,17 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     plan->shape = *sh;
     plan->n_items16 = static_cast<uint32_t>(t.items16.size());
     plan->n_tc_ctas = static_cast<uint32_t>(t.tc_ptr.size()) - 1;
-    plan->merge = t.needs_merge;
     plan->n_prefix_pages = prefix_indptr[NG];
     plan->n_suffix_pages = suffix_indptr[B];
     PrefixArgs& a = plan->base;
     a.lists = reinterpret_cast<const PrefixList*>(base + o_lists);
     a.tiles = reinterpret_cast<const PrefixTile*>(base + o_tiles);
     a.items = reinterpret_cast<const PrefixItem*>(base + o_items);
-    a.tc_items = reinterpret_cast<const PrefixItem*>(base + o_tc);
+    a.tc_items = reinterpret_cast<const PrefixTcItem*>(base + o_tc);
     a.tc_ptr = reinterpret_cast<const uint32_t*>(base + o_ptr);
     a.row_tok = reinterpret_cast<const uint32_t*>(base + o_row);
-    a.tok_lists = reinterpret_cast<const uint4*>(base + o_tok);
+    a.merge_rows = reinterpret_cast<const PrefixMergeRow*>(base + o_merge);
+    a.n_merge = static_cast<uint32_t>(t.merge_rows.size());
     a.status = reinterpret_cast<uint32_t*>(base + o_status);
     a.part_ml = reinterpret_cast<float2*>(base + o_ml);
     a.part_o = reinterpret_cast<float*>(base + o_o);
@@ -2136,7 +2129,7 @@ void weaver_prefix_plan_destroy(weaver_prefix_plan* plan) {
 
 int weaver_prefix_plan_kernel_count(const weaver_prefix_plan* plan) {
     if (!plan) return 0;
-    return (plan->n_tc_ctas ? 1 : 0) + (plan->n_items16 ? 1 : 0) + (plan->merge ? 1 : 0);
+    return (plan->n_tc_ctas ? 1 : 0) + (plan->n_items16 ? 1 : 0) + (plan->base.n_merge ? 1 : 0);
 }
 
 int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, void* stream) {
@@ -2188,7 +2181,7 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
         WEAVER_CUDA_TRY(launch_prefix_tc(a, tm_k, tm_v, plan->n_tc_ctas, s), "prefix attention launch");
     }
     if (plan->n_items16) WEAVER_CUDA_TRY(launch_prefix_rows16(a, plan->n_items16, s), "prefix attention launch");
-    if (plan->merge) WEAVER_CUDA_TRY(launch_prefix_merge(a, s), "prefix merge launch");
+    if (a.n_merge) WEAVER_CUDA_TRY(launch_prefix_merge(a, s), "prefix merge launch");
     return WEAVER_OK;
 }
 

@@ -351,21 +351,40 @@ struct PrefixList {
     uint32_t tile0, n_tiles, tile_rows;      // first tile; row tiles per kv head; rows of a tile
     uint32_t causal;                         // of the own pages
 };
-// Rows row0 .. of one list's rows of one kv head.  Its partials are n_slots
-// runs of its rows from part_row0.
+// Rows row0 .. row0 + rows - 1 of one list's rows of one kv head.  Its partials
+// are n_slots runs of its rows from part_row0; a run holds its rows' sums as
+// [D / 4][rows][4] floats from part_row * D, so that a thread per row stores 16
+// bytes next to its neighbour's.
 struct PrefixTile {
     uint64_t part_row0;
-    uint32_t list, kvh, row0;
+    uint32_t list, kvh, row0, rows;
     uint32_t n_slots, direct;  // direct: its only item writes the output
-    uint32_t pad;
 };
-// Pages blk0 .. blk1-1 of a tile's list (16-row tiles), or 128-token tiles of
-// pages blk0 .. blk1-1 (tensor-memory tiles), counted over the prefix's pages
+// Pages blk0 .. blk1-1 of a 16-row tile's list, counted over the prefix's pages
 // and then the own ones.
 struct PrefixItem {
     uint64_t part_row;
-    uint32_t tile, blk0, blk1;
-    uint32_t two;  // tensor-memory tiles of at most 128 rows: the two halves of the CTA write a slot each
+    uint32_t tile, blk0, blk1, pad;
+};
+// Token tiles t0 .. t1-1 (kTcPages pages each) of a tensor-memory tile's list (the prefix's
+// pre_tiles, then the own pages'), with all that the kernel needs of the tile
+// and the list: read by one warp-wide load.
+struct PrefixTcItem {
+    uint64_t part_row;
+    uint32_t tok0, row0, rows, kvh, ntok;
+    uint32_t pre_ref0, pre_blocks, pre_len, pre_tiles;
+    uint32_t suf_ref0, suf_blocks, suf_len;
+    uint32_t t0, t1;
+    uint32_t flags;  // kTcCausal, kTcTwo, kTcDirect
+    uint32_t pad[3];
+};
+constexpr uint32_t kTcPages = 4;  // pages of a token tile: 64 tokens
+constexpr uint32_t kTcCausal = 1, kTcDirect = 2;
+constexpr uint32_t kTcTwo = 4;  // at most 128 rows and several token tiles: the two halves of the CTA write a slot each
+static_assert(sizeof(PrefixTcItem) == 80, "one word per lane of a warp");
+// One output row to be merged from its rows of up to two tiles (~0: none).
+struct PrefixMergeRow {
+    uint32_t out_row, tile[2], row[2];
 };
 struct PrefixArgs {
     const __half *q, *k, *v;
@@ -375,16 +394,16 @@ struct PrefixArgs {
     const uint32_t *prefix_lens, *suffix_lens;  // null: every page is full
     uint64_t pool_blocks;
     const PrefixItem* items;           // of the 16-row tiles
-    const PrefixItem* tc_items;        // of the tensor-memory tiles, CTA c's are [tc_ptr[c], tc_ptr[c+1])
+    const PrefixTcItem* tc_items;      // of the tensor-memory tiles, CTA c's are [tc_ptr[c], tc_ptr[c+1])
     const uint32_t* tc_ptr;
     const PrefixTile* tiles;
     const PrefixList* lists;
     const uint32_t* row_tok;
-    const uint4* tok_lists;            // [tokens] (list, token of it) of its prefix part, of its own part; ~0: none
+    const PrefixMergeRow* merge_rows;
     float2* part_ml;
     float* part_o;
     uint32_t* status;
-    uint32_t n_tokens, Hq, Hkv, G, D;
+    uint32_t n_tokens, n_merge, Hq, Hkv, G, D;
     float scale;
 };
 // The host's view of a plan's geometry and the tables made from it.
@@ -396,11 +415,11 @@ struct PrefixGeometry {
 struct PrefixTables {
     std::vector<PrefixList> lists;
     std::vector<PrefixTile> tiles;
-    std::vector<PrefixItem> items16, items_tc;
+    std::vector<PrefixItem> items16;
+    std::vector<PrefixTcItem> items_tc;
     std::vector<uint32_t> tc_ptr, row_tok;
-    std::vector<uint4> tok_lists;
+    std::vector<PrefixMergeRow> merge_rows;
     uint64_t part_rows = 0;
-    bool needs_merge = false;
 };
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t);
 cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s);

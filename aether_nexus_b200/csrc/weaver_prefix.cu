@@ -64,9 +64,6 @@ __device__ __forceinline__ void px_issue(uint8_t* st, const PrefixArgs& a, uint6
     }
 }
 
-// 1 / l; 0 for a row that saw nothing; NaN stays NaN.
-__device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); }
-
 template <int D>
 __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixArgs a) {
     using L = PxLayout<D>;
@@ -80,9 +77,9 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
     const PrefixItem it = a.items[blockIdx.x];
     const PrefixTile tile = a.tiles[it.tile];
     const PrefixList list = a.lists[tile.list];
-    const uint32_t g = tile.kvh, R = list.ntok * a.G;
-    const uint32_t rows = min(16u, R - tile.row0);
-    const uint32_t pre_len = prefix_len(a, list, tid == 0), suf_len = suffix_len(a, list, tid == 0);
+    const uint32_t g = tile.kvh, rows = tile.rows;
+    const uint32_t pre_len = page_len(a.prefix_lens, list.pre_len, list.pre_blocks, a.status, tid == 0);
+    const uint32_t suf_len = page_len(a.suffix_lens, list.suf_len, list.suf_blocks, a.status, tid == 0);
     auto out_row = [&](uint32_t r) {  // row r of the tile in q and out
         const uint32_t rr = tile.row0 + r, j = rr / a.G;
         return static_cast<uint64_t>(a.row_tok[list.tok0 + j]) * a.Hq + g * a.G + (rr - j * a.G);
@@ -102,11 +99,11 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
     for (int hh = 0; hh < 2; ++hh) {
         const uint32_t r = gid + 8 * hh;
         lim_pre[hh] = r < rows ? static_cast<int32_t>(pre_len) : 0;
-        lim_suf[hh] = r < rows ? static_cast<int32_t>(suffix_limit(list, suf_len, (tile.row0 + r) / a.G)) : 0;
+        lim_suf[hh] = r < rows ? static_cast<int32_t>(suffix_limit(list.causal, suf_len, list.ntok, (tile.row0 + r) / a.G)) : 0;
     }
     // the item's pages below the lengths and the tile's largest limit: n_pre of
     // the prefix from blk0, then own ones from suf0; this warp takes every fourth
-    const uint32_t top = suffix_limit(list, suf_len, (tile.row0 + rows - 1) / a.G);
+    const uint32_t top = suffix_limit(list.causal, suf_len, list.ntok, (tile.row0 + rows - 1) / a.G);
     const uint32_t p1 = min(it.blk1, (pre_len + kBlock - 1) / kBlock);
     const uint32_t n_pre = p1 > it.blk0 ? p1 - it.blk0 : 0;
     const uint32_t suf0 = it.blk0 > list.pre_blocks ? it.blk0 - list.pre_blocks : 0;
@@ -151,7 +148,8 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
     fa_store_partial<D>(red + warp * 16 * (D + 2), m_run, l_run, o, lane);
     __syncthreads();
     for (uint32_t x = tid; x < 16 * D; x += kPxThreads) {
-        const uint32_t r = x / D, d = x % D;
+        // four dimensions of a row to each quad of threads, the next row to the next quad
+        const uint32_t r = (x / 4) % 16, d = x / 64 * 4 + x % 4;
         if (r >= rows) continue;
         float M = -INFINITY;
 #pragma unroll
@@ -167,79 +165,53 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
         if (tile.direct) {
             a.out[out_row(r) * D + d] = __float2half_rn(O * inverse_sum(Lsum));
         } else {
-            const uint64_t row = it.part_row + static_cast<uint64_t>(r);
-            if (d == 0) a.part_ml[row] = make_float2(M, Lsum);
-            a.part_o[row * D + d] = O;
+            if (d == 0) a.part_ml[it.part_row + r] = make_float2(M, Lsum);
+            a.part_o[it.part_row * D + (d / 4 * rows + r) * 4 + d % 4] = O;
         }
     }
 }
 
-// One warp per (query token, q head): the parts of its pooled tile and of its
-// own tile.
+// A thread per (merged row, four dimensions), rows fastest: one pass over the
+// slots of the row's tiles with the running maximum.
 template <int D>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
-    constexpr int V = D / 32;  // elements per lane
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31;
-    if (row >= static_cast<uint64_t>(a.n_tokens) * a.Hq) return;
-    const uint32_t t = static_cast<uint32_t>(row / a.Hq), h = static_cast<uint32_t>(row % a.Hq), g = h / a.G;
-    const uint4 at = a.tok_lists[t];
-    uint64_t base[2];
-    uint32_t n[2], step[2];
+    constexpr uint32_t kRows = 8;  // neighbouring rows per run of D / 4 threads each
+    const uint64_t idx = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint64_t i = idx / (kRows * D / 4) * kRows + idx % kRows;
+    const uint32_t c = static_cast<uint32_t>(idx / kRows % (D / 4));
+    if (i >= a.n_merge) return;
+    const PrefixMergeRow mr = a.merge_rows[i];
+    float M = -INFINITY, L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        n[s] = 0;
-        base[s] = 0;
-        step[s] = 0;
-        const uint32_t list = s ? at.z : at.x;
-        if (list == ~0u) continue;
-        const PrefixList L = a.lists[list];
-        if (L.pre_blocks + L.suf_blocks == 0) continue;
-        const uint32_t rr = (s ? at.w : at.y) * a.G + h % a.G;
-        const PrefixTile T = a.tiles[L.tile0 + g * L.n_tiles + rr / L.tile_rows];
-        if (T.direct) return;  // its only item wrote the output
-        n[s] = T.n_slots;
-        step[s] = min(L.tile_rows, L.ntok * a.G - T.row0);
-        base[s] = T.part_row0 + (rr - T.row0);
-    }
-    float M = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-        for (uint32_t i = lane; i < n[s]; i += 32) M = fmaxf(M, a.part_ml[base[s] + static_cast<uint64_t>(i) * step[s]].x);
-    M = warp_max(M);
-    float Lsum = 0.0f, O[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) O[v] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
+        if (mr.tile[s] == ~0u) continue;
+        const PrefixTile T = a.tiles[mr.tile[s]];
+        const float2* ml = a.part_ml + T.part_row0 + mr.row[s];
+        const float4* o = reinterpret_cast<const float4*>(a.part_o + T.part_row0 * D) + c * T.rows + mr.row[s];
 #pragma unroll 4
-        for (uint32_t i = 0; i < n[s]; ++i) {
-            const uint64_t p = base[s] + static_cast<uint64_t>(i) * step[s];
-            const float2 ml = a.part_ml[p];
-            const float f = exp_shift(ml.x, M);
-            Lsum += ml.y * f;
-            if (V == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(a.part_o + p * D + lane * 4);
-                O[0] += x.x * f, O[1] += x.y * f, O[2 % V] += x.z * f, O[3 % V] += x.w * f;
-            } else {
-                const float2 x = *reinterpret_cast<const float2*>(a.part_o + p * D + lane * 2);
-                O[0] += x.x * f, O[1] += x.y * f;
-            }
+        for (uint32_t k = 0; k < T.n_slots; ++k) {
+            const float2 x = ml[static_cast<uint64_t>(k) * T.rows];
+            const float4 y = o[static_cast<uint64_t>(k) * T.rows * (D / 4)];
+            const float Mn = fmaxf(M, x.x);
+            const float f0 = exp_shift(M, Mn), f1 = exp_shift(x.x, Mn);
+            M = Mn;
+            L = L * f0 + x.y * f1;
+            O = make_float4(O.x * f0 + y.x * f1, O.y * f0 + y.y * f1, O.z * f0 + y.z * f1, O.w * f0 + y.w * f1);
         }
     }
+    const uint64_t row = mr.out_row;
     if (a.out_m) {
-        if (lane == 0) {
+        if (c == 0) {
             a.out_m[row] = M;
-            a.out_l[row] = Lsum;
+            a.out_l[row] = L;
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) a.out_o[row * D + lane * V + v] = O[v];
+        *reinterpret_cast<float4*>(a.out_o + row * D + c * 4) = O;
         return;
     }
-    const float inv = inverse_sum(Lsum);
-#pragma unroll
-    for (int v = 0; v < V; v += 2)
-        *reinterpret_cast<__half2*>(a.out + row * D + lane * V + v) = __floats2half2_rn(O[v] * inv, O[v + 1] * inv);
+    const float inv = inverse_sum(L);
+    __half2 h[2] = {__floats2half2_rn(O.x * inv, O.y * inv), __floats2half2_rn(O.z * inv, O.w * inv)};
+    *reinterpret_cast<uint2*>(a.out + row * D + c * 4) = *reinterpret_cast<const uint2*>(h);
 }
 
 }  // namespace
@@ -248,12 +220,16 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
 // its own over prefix and own pages: its padding to 128 rows is at most a
 // quarter then, and it saves writing and reading two partials a row.
 constexpr uint32_t kOwnRows = 512;
+// Starting an item (query rows in, results out, the pipeline filling) in the
+// units of a token tile's cost.
+constexpr uint32_t kItemCost = 24;
 // Up to 16 rows a 16-row tile costs one pass over the pages either way.
 constexpr uint32_t kRows16 = 16;
 
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     const uint32_t G = geo.Hq / geo.Hkv, NG = geo.n_groups, B = geo.n_seqs, none = ~0u;
-    t->tok_lists.assign(geo.q_indptr[B], uint4{none, 0, none, 0});
+    // (list, token of it) of every token's pooled part and of its own part
+    std::vector<uint4> at(geo.q_indptr[B], uint4{none, 0, none, 0});
     for (uint32_t i = 0; i < NG; ++i) {
         const uint32_t s0 = geo.group_indptr[i], s1 = geo.group_indptr[i + 1];
         const uint32_t pre0 = geo.prefix_indptr[i], pre_blocks = geo.prefix_indptr[i + 1] - pre0;
@@ -271,8 +247,8 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
             for (uint32_t b = s0; b < s1; ++b)
                 if (few(b))
                     for (uint32_t q = geo.q_indptr[b]; q < geo.q_indptr[b + 1]; ++q) {
-                        t->tok_lists[q].x = static_cast<uint32_t>(t->lists.size());
-                        t->tok_lists[q].y = L.ntok++;
+                        at[q].x = static_cast<uint32_t>(t->lists.size());
+                        at[q].y = L.ntok++;
                         t->row_tok.push_back(q);
                     }
             t->lists.push_back(L);
@@ -291,8 +267,8 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
             L.suf_len = b;
             L.causal = geo.causal ? 1u : 0u;
             for (uint32_t q = geo.q_indptr[b]; q < geo.q_indptr[b + 1]; ++q) {
-                t->tok_lists[q].z = static_cast<uint32_t>(t->lists.size());
-                t->tok_lists[q].w = L.ntok++;
+                at[q].z = static_cast<uint32_t>(t->lists.size());
+                at[q].w = L.ntok++;
                 t->row_tok.push_back(q);
             }
             t->lists.push_back(L);
@@ -303,12 +279,8 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     auto rows_of = [&](uint32_t l) { return static_cast<uint64_t>(t->lists[l].ntok) * G; };
     // lists whose rows get something from another list too
     std::vector<uint8_t> joined(n_lists, geo.partials ? 1 : 0);
-    t->needs_merge = geo.partials && geo.q_indptr[B];
-    for (const uint4& x : t->tok_lists) {
-        const bool p = x.x != none && pages(x.x), o = x.z != none && pages(x.z);
-        if (p && o) joined[x.x] = joined[x.z] = 1;
-        if (!p && !o) t->needs_merge = true;  // its zeros come from the merge
-    }
+    for (const uint4& x : at)
+        if (x.x != none && pages(x.x) && x.z != none && pages(x.z)) joined[x.x] = joined[x.z] = 1;
 
     // tiles, and the work of either kind
     struct TcTile { uint32_t tile, n, cost; };
@@ -328,33 +300,30 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
                 T.list = l;
                 T.kvh = g;
                 T.row0 = r * L.tile_rows;
+                T.rows = static_cast<uint32_t>(std::min<uint64_t>(L.tile_rows, rows_of(l) - T.row0));
                 if (small) {
                     work16 += pages(l);
                 } else {
-                    // 128-token tiles below the causal limit of the tile's last
+                    // token tiles below the causal limit of the tile's last
                     // row, the pages taken as full
-                    const uint64_t rows = std::min<uint64_t>(256, rows_of(l) - T.row0);
                     uint64_t own = static_cast<uint64_t>(L.suf_blocks) * kBlock;
                     if (L.causal) {
-                        const int64_t lim = static_cast<int64_t>(own) - L.ntok + 1 + (T.row0 + rows - 1) / G;
+                        const int64_t lim = static_cast<int64_t>(own) - L.ntok + 1 + (T.row0 + T.rows - 1) / G;
                         own = lim > 0 ? std::min<uint64_t>(own, lim) : 0;
                     }
-                    const uint32_t n = static_cast<uint32_t>((L.pre_blocks + 7) / 8 + (own + 127) / 128);
+                    const uint32_t n = static_cast<uint32_t>((L.pre_blocks + kTcPages - 1) / kTcPages +
+                                                             (own + kTcPages * kBlock - 1) / (kTcPages * kBlock));
                     // a token tile of 256 rows keeps the exponentials busy for two
                     // tiles of 128, one of fewer rows waits for HBM
-                    const uint32_t cost = rows > 128 ? 8 : 5;
+                    const uint32_t cost = T.rows > 128 ? 8 : 5;
                     tc.push_back(TcTile{static_cast<uint32_t>(t->tiles.size()), std::max(n, 1u), cost});
-                    cost_tc += static_cast<uint64_t>(tc.back().n) * cost;
+                    cost_tc += static_cast<uint64_t>(tc.back().n) * cost + kItemCost;
                     n_tc += tc.back().n;
                 }
                 t->tiles.push_back(T);
             }
     }
     uint64_t part_rows = 0;
-    auto tile_rows = [&](const PrefixTile& T) {
-        const PrefixList& L = t->lists[T.list];
-        return std::min<uint64_t>(L.tile_rows, rows_of(T.list) - T.row0);
-    };
 
     // 16-row tiles: about three CTAs fit an SM; items of whole multiples of
     // four pages (one per warp), as long as that still gives two full waves
@@ -363,7 +332,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     for (uint32_t ti = 0; ti < t->tiles.size(); ++ti) {
         PrefixTile& T = t->tiles[ti];
         if (t->lists[T.list].tile_rows != 16) continue;
-        const uint64_t n = pages(T.list), rows = tile_rows(T);
+        const uint64_t n = pages(T.list), rows = T.rows;
         T.n_slots = static_cast<uint32_t>((n + per - 1) / per);
         T.direct = T.n_slots == 1 && !joined[T.list];
         T.part_row0 = part_rows;
@@ -375,9 +344,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
             it.part_row = part_rows + s * rows;
             t->items16.push_back(it);
         }
-        if (T.direct) continue;
-        part_rows += T.n_slots * rows;
-        t->needs_merge = true;
+        if (!T.direct) part_rows += T.n_slots * rows;
     }
 
     // tensor-memory tiles: one CTA per SM, each with an equal share of the
@@ -388,8 +355,10 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     uint32_t cta = 0;
     for (const TcTile& x : tc) {
         PrefixTile& T = t->tiles[x.tile];
-        const uint64_t rows = tile_rows(T);
+        const PrefixList& L = t->lists[T.list];
+        const size_t first = t->items_tc.size();
         T.part_row0 = part_rows;
+        spent += kItemCost;
         for (uint32_t b = 0; b < x.n;) {
             const uint64_t end = cost_tc * (cta + 1) / n_ctas;  // this CTA's share ends here
             uint64_t take = (end > spent ? end - spent : 0) / x.cost;
@@ -401,24 +370,47 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
                 continue;
             }
             take = std::min<uint64_t>(take, x.n - b);
-            PrefixItem it{};
-            it.tile = x.tile;
-            it.blk0 = b;
-            it.blk1 = static_cast<uint32_t>(b + take);
-            it.two = rows <= 128 && take > 1;
-            it.part_row = part_rows + T.n_slots * rows;
-            T.n_slots += it.two ? 2 : 1;
+            PrefixTcItem it{};
+            it.part_row = part_rows + static_cast<uint64_t>(T.n_slots) * T.rows;
+            it.tok0 = L.tok0, it.row0 = T.row0, it.rows = T.rows, it.kvh = T.kvh, it.ntok = L.ntok;
+            it.pre_ref0 = L.pre_ref0, it.pre_blocks = L.pre_blocks, it.pre_len = L.pre_len;
+            it.pre_tiles = (L.pre_blocks + kTcPages - 1) / kTcPages;
+            it.suf_ref0 = L.suf_ref0, it.suf_blocks = L.suf_blocks, it.suf_len = L.suf_len;
+            it.t0 = b;
+            it.t1 = static_cast<uint32_t>(b + take);
+            const bool two = T.rows <= 128 && take > 1;
+            it.flags = (L.causal ? kTcCausal : 0) | (two ? kTcTwo : 0);
+            T.n_slots += two ? 2 : 1;
             t->items_tc.push_back(it);
             b += static_cast<uint32_t>(take);
             spent += take * x.cost;
         }
         T.direct = T.n_slots == 1 && !joined[T.list];
-        if (T.direct) continue;
-        part_rows += T.n_slots * rows;
-        t->needs_merge = true;
+        if (T.direct)
+            t->items_tc[first].flags |= kTcDirect;
+        else
+            part_rows += static_cast<uint64_t>(T.n_slots) * T.rows;
     }
     if (!tc.empty()) t->tc_ptr.push_back(static_cast<uint32_t>(t->items_tc.size()));
     t->part_rows = part_rows;
+
+    // the rows that no single item writes, those with nothing to attend to
+    // (their zeros) included
+    for (uint32_t q = 0; q < geo.q_indptr[B]; ++q)
+        for (uint32_t h = 0; h < geo.Hq; ++h) {
+            PrefixMergeRow m{q * geo.Hq + h, {none, none}, {0, 0}};
+            const uint32_t list[2] = {at[q].x, at[q].z}, tok[2] = {at[q].y, at[q].w};
+            bool direct = false;
+            for (int s = 0; s < 2; ++s) {
+                if (list[s] == none || !pages(list[s])) continue;
+                const PrefixList& L = t->lists[list[s]];
+                const uint32_t r = tok[s] * G + h % G;
+                m.tile[s] = L.tile0 + h / G * L.n_tiles + r / L.tile_rows;
+                m.row[s] = r % L.tile_rows;
+                direct |= t->tiles[m.tile[s]].direct != 0;
+            }
+            if (!direct) t->merge_rows.push_back(m);
+        }
 }
 
 namespace {
@@ -440,7 +432,7 @@ cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStre
 }
 
 cudaError_t launch_prefix_merge(const PrefixArgs& a, cudaStream_t s) {
-    const uint32_t grid = static_cast<uint32_t>((static_cast<uint64_t>(a.n_tokens) * a.Hq + 7) / 8);
+    const uint32_t grid = static_cast<uint32_t>((a.n_merge + 7ull) / 8 * 8 * (a.D / 4) / 256) + 1;
     if (a.D == 128)
         prefix_merge_kernel<128><<<grid, 256, 0, s>>>(a);
     else

@@ -15,19 +15,16 @@ __device__ __forceinline__ uint32_t page_len(const uint32_t* lens, uint32_t i, u
     if (n > cap && report) atomicOr(status, DEVERR_REF_RANGE);
     return min(n, cap);
 }
-__device__ __forceinline__ uint32_t prefix_len(const PrefixArgs& a, const PrefixList& L, bool report) {
-    return page_len(a.prefix_lens, L.pre_len, L.pre_blocks, a.status, report);
-}
-__device__ __forceinline__ uint32_t suffix_len(const PrefixArgs& a, const PrefixList& L, bool report) {
-    return page_len(a.suffix_lens, L.suf_len, L.suf_blocks, a.status, report);
-}
 
-// Own tokens that query j of the list's ntok sees: all, or with the causal
-// rule len - ntok + 1 + j of them.
-__device__ __forceinline__ uint32_t suffix_limit(const PrefixList& L, uint32_t len, uint32_t j) {
-    if (!L.causal) return len;
-    const int64_t lim = static_cast<int64_t>(len) - L.ntok + 1 + j;
+// Own tokens that query j of ntok sees: all, or with the causal rule len -
+// ntok + 1 + j of them.
+__device__ __forceinline__ uint32_t suffix_limit(bool causal, uint32_t len, uint32_t ntok, uint32_t j) {
+    if (!causal) return len;
+    const int64_t lim = static_cast<int64_t>(len) - ntok + 1 + j;
     return lim > 0 ? static_cast<uint32_t>(lim) : 0u;
 }
+
+// 1 / l; 0 for a row that saw nothing; NaN stays NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); }
 
 }  // namespace weaver

@@ -2,7 +2,7 @@
 // 5th-generation tensor cores.
 //
 // One persistent CTA per SM works through its items; an item is a tile of up
-// to 256 query rows of one kv head against a run of 128-token tiles of its
+// to 256 query rows of one kv head against a run of 64-token tiles of its
 // page list (the group's prefix pages, then the sequence's own).  Two halves
 // of the CTA run the online softmax, one thread per row:
 //   S = Q K^T (tcgen05.mma, Q and K in shared memory, S in tensor memory)
@@ -10,24 +10,29 @@
 //   O += P V (P from tensor memory, V in shared memory)
 // A tile of more than 128 rows gives each half 128 rows of it and both take
 // every token tile; a smaller one gives both halves the same rows and every
-// other token tile, so the exponentials of one half overlap the products of the
-// other either way.  m is the row's maximum up to 2^8: the accumulator is
+// other token tile.  m is the row's maximum up to 2^8: the accumulator is
 // rescaled only when the maximum has grown by more than that, since p <= 2^8
 // and its f16 rounding is relative.
 //
-// Tensor memory (512 columns): S of either half (128 each; P lies in its first
-// 64), O of either half (D each).  Pages arrive by one TMA box per page and
-// tensor, [2 groups of 8 rows][D/64 halves][8 rows][128 B]: K is a K-major
+// Tensor memory (512 columns): two S of either half (64 columns each; P lies
+// in the first 32), O of either half (D each).  With two S the product for the
+// tile after next is issued when P of this one has been used, so the softmax
+// finds its next S ready: with one S of 128 tokens each half waited out P V
+// and Q K of its own before its next tile (5400 clocks for a 256 x 128 tile,
+// against 2048 of the exponential unit).  Pages arrive by one TMA box per page
+// and tensor, [2 groups of 8 rows][D/64 halves][8 rows][128 B]: K is a K-major
 // operand with 8-row groups D * 16 bytes apart, V an MN-major one whose 16
 // tokens per step are one page.
 //
 // Warps 0-3 and 4-7: the halves; warp 8: MMA; warp 9: TMA; warps 10 and 11
 // only complete the third warpgroup, whose registers the first two take over
 // (launched with 168 a thread: 384 * 168 = 64512 >= 256 * 216 + 128 * 64).
+// Code that runs once per item is kept in rolled loops: the first pass over
+// straight-line code is bound by instruction fetch (10 us for an unrolled copy
+// of the query tile).
 //
 // Bound: up to about 250 rows per kv head by HBM (D * 4 bytes a token and kv
-// head); above that by the exponential unit and the tensor cores, which need
-// the same 2048 clocks per 256 x 128 tile at D = 128.
+// head); above that by the exponential unit and the tensor cores.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -40,8 +45,8 @@ namespace weaver {
 namespace {
 
 constexpr uint32_t kTcThreads = 384;  // three warpgroups
-constexpr uint32_t kTileTokens = 128;
-constexpr uint32_t kTilePages = kTileTokens / kBlock;
+constexpr uint32_t kTilePages = kTcPages;
+constexpr uint32_t kTileTokens = kTilePages * kBlock;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.0f;  // log2 of the growth of the maximum that forces a rescale
@@ -49,17 +54,19 @@ constexpr float kRescale = 8.0f;  // log2 of the growth of the maximum that forc
 template <int D>
 struct TcLayout {
     static constexpr uint32_t kPage = kBlock * D * 2;
-    static constexpr uint32_t kBuf = kTileTokens * D * 2;  // 128 tokens of K (or V)
-    static constexpr uint32_t kBufs = D == 128 ? 5 : 10;   // ring of buffers, K and V in turn
+    static constexpr uint32_t kBuf = kTileTokens * D * 2;  // one token tile of K (or V)
+    static constexpr uint32_t kBufs = D == 128 ? 10 : 20;  // ring of buffers, K and V in turn
     static constexpr uint32_t kQ = 128 * D * 2;
     static constexpr uint32_t kBytes = 2 * kQ + kBufs * kBuf;
     static constexpr uint32_t kO = 256;                    // tensor-memory column of the first accumulator
 };
 
 struct TcBars {
-    uint64_t full[10], empty[10];
-    uint64_t q_full[2], s_full[2], p_ready[2], o_done[2];
-    uint64_t drain;
+    uint64_t full[20], empty[20];
+    // [half][tile of the half & 1]: the products of two tiles of a half may be
+    // outstanding, and a parity tells only neighbouring phases apart
+    uint64_t q_full[2], s_full[2][2], p_ready[2][2], o_done[2][2];
+    uint64_t tail, drain;
     uint32_t tmem;
 };
 
@@ -78,29 +85,30 @@ __device__ __forceinline__ bool row_wait(uint64_t* bar, uint32_t parity, uint32_
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, site));
 }
 
-// Shared-memory matrix descriptor, 128-byte swizzle (atoms of 8 x 128 bytes).
+// Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 x 128 bytes).
 // K-major: sbo = bytes between 8-row groups (lbo unused).  MN-major: lbo =
-// bytes between 64-element column groups, sbo = between 8-row groups.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-           (static_cast<uint64_t>(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// bytes between 64-element column groups, sbo = between 8-row groups.  The low
+// word holds address and lbo, the high word is a constant of the layout.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | (lbo >> 4 << 16); }
+constexpr uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | (1u << 14) | (2u << 29); }
 // kind::f16, f16 operands, fp32 accumulators; b_mn: B is MN-major.
 constexpr uint32_t f16_idesc(uint32_t M, uint32_t N, uint32_t b_mn) {
     return (1u << 4) | (b_mn << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+template <uint32_t kHiA, uint32_t kHiB>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %6};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kHiA), "n"(kHiB)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+template <uint32_t kHiB>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kHiB)
         : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -109,19 +117,38 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 lanes x 32 columns, this lane's row.
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t r[32]) {
+// 32 lanes x 32 (64) columns, this lane's row.  The wait is part of the
+// statement: nothing that uses the values can be moved before it.
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float r[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_ld64(uint32_t taddr, float r[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+          "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+          "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+          "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+          "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t r[32]) {
@@ -134,6 +161,36 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t r[32]) {
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const float r[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+        "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
+        "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
+        "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31])
+        : "memory");
+}
+
+// Two fp32 lanes per instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -153,45 +210,63 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-// What an item comes to, the same for every role.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// What an item comes to, the same for every role; every value is the same in
+// all lanes of the warp, by shuffle, so that the MMA operands stay in uniform
+// registers (a thread that feeds them from its own registers issues an MMA at
+// half the rate at which the tensor cores take it).
 struct Work {
-    PrefixItem it;
-    PrefixTile tile;
-    PrefixList list;
-    uint32_t R, rows;            // rows of the kv head, of this tile
+    uint64_t part_row;
+    uint32_t tok0, row0, rows, kvh, ntok, flags;
+    uint32_t pre_ref, suf_ref;   // first page of the lists
     uint32_t pre_len, suf_len;
     uint32_t pre0, n_pre, suf0;  // token tiles: n_pre of the prefix from pre0, then own ones from suf0
     uint32_t n;                  // token tiles in all
-    bool pair;                   // each half has rows of its own
+    bool pair;                   // more than 128 rows: each half of the CTA has rows of its own
 
-    __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t item, bool report) {
-        it = a.tc_items[item];
-        tile = a.tiles[it.tile];
-        list = a.lists[tile.list];
-        R = list.ntok * a.G;
-        rows = min(256u, R - tile.row0);
+    // This lane's word of item i's record.
+    static __device__ __forceinline__ uint32_t fetch(const PrefixArgs& a, uint32_t i, uint32_t end, uint32_t lane) {
+        return i < end && lane < sizeof(PrefixTcItem) / 4 ? reinterpret_cast<const uint32_t*>(a.tc_items + i)[lane] : 0u;
+    }
+    __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t word, bool report) {
+        auto at = [&](uint32_t w) { return __shfl_sync(0xffffffffu, word, w); };
+        part_row = static_cast<uint64_t>(at(1)) << 32 | at(0);
+        tok0 = at(2), row0 = at(3), rows = at(4), kvh = at(5), ntok = at(6);
+        pre_ref = at(7);
+        const uint32_t pre_blocks = at(8), pre_i = at(9), cap = at(10);
+        suf_ref = at(11);
+        const uint32_t suf_blocks = at(12), suf_i = at(13), t0 = at(14), t1 = at(15);
+        flags = at(16);
         pair = rows > 128;
-        pre_len = prefix_len(a, list, report);
-        suf_len = suffix_len(a, list, report);
+        pre_len = __shfl_sync(0xffffffffu, page_len(a.prefix_lens, pre_i, pre_blocks, a.status, report), 0);
+        suf_len = __shfl_sync(0xffffffffu, page_len(a.suffix_lens, suf_i, suf_blocks, a.status, report), 0);
         // own tokens below the largest limit of the tile's rows
-        const uint32_t top = suffix_limit(list, suf_len, (tile.row0 + rows - 1) / a.G);
-        const uint32_t cap = (list.pre_blocks + kTilePages - 1) / kTilePages;  // prefix tiles counted by the plan
-        const uint32_t p1 = min(it.blk1, (pre_len + kTileTokens - 1) / kTileTokens);
-        pre0 = it.blk0;
+        const uint32_t top = limit((row0 + rows - 1) / a.G);
+        const uint32_t p1 = min(t1, (pre_len + kTileTokens - 1) / kTileTokens);
+        pre0 = t0;
         n_pre = p1 > pre0 ? p1 - pre0 : 0;
-        suf0 = it.blk0 > cap ? it.blk0 - cap : 0;
-        const uint32_t s1 = min(it.blk1 > cap ? it.blk1 - cap : 0, (top + kTileTokens - 1) / kTileTokens);
+        suf0 = t0 > cap ? t0 - cap : 0;
+        const uint32_t s1 = min(t1 > cap ? t1 - cap : 0, (top + kTileTokens - 1) / kTileTokens);
         n = n_pre + (s1 > suf0 ? s1 - suf0 : 0);
     }
+    __device__ __forceinline__ uint32_t limit(uint32_t j) const { return suffix_limit(flags & kTcCausal, suf_len, ntok, j); }
     // token tiles of half h
     __device__ __forceinline__ uint32_t count(uint32_t h) const { return pair ? n : (n + 1 - h) / 2; }
     __device__ __forceinline__ uint32_t tile_of(uint32_t j, uint32_t h) const { return pair ? j : 2 * j + h; }
-    // token tile t: whether of the own pages, its first token there, tokens of the list from it on
+    // token tile t: whether of the own pages, its first token there, tokens of the list, its first page reference
     __device__ __forceinline__ bool own(uint32_t t) const { return t >= n_pre; }
     __device__ __forceinline__ uint32_t first(uint32_t t) const {
         return (own(t) ? suf0 + (t - n_pre) : pre0 + t) * kTileTokens;
     }
     __device__ __forceinline__ uint32_t length(uint32_t t) const { return own(t) ? suf_len : pre_len; }
+    __device__ __forceinline__ const uint32_t* refs(const PrefixArgs& a, uint32_t t) const {
+        return (own(t) ? a.suffix_refs + suf_ref : a.prefix_refs + pre_ref) + first(t) / kBlock;
+    }
 };
 
 template <int D>
@@ -221,212 +296,241 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         }
         for (uint32_t h = 0; h < 2; ++h) {
             mbar_init(&bars.q_full[h], 128);
-            mbar_init(&bars.s_full[h], 1);
-            mbar_init(&bars.p_ready[h], 4);
-            mbar_init(&bars.o_done[h], 1);
+            for (uint32_t b = 0; b < 2; ++b) {
+                mbar_init(&bars.s_full[h][b], 1);
+                mbar_init(&bars.p_ready[h][b], 4);
+                mbar_init(&bars.o_done[h][b], 1);
+            }
         }
+        mbar_init(&bars.tail, 1);
         mbar_init(&bars.drain, 1);
         fence_barrier_init();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bars.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
+    uint32_t word = Work::fetch(a, i0, i1, lane);  // the next item's record
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 9) {
             // ---- TMA: K and V of every token tile, in turn, into the ring
             bool ok = true;
-            uint32_t c_full = 0;  // buffers filled so far
+            uint32_t b = 0, fill = 0;  // next buffer; how often the ring has been filled
+            uint32_t n_tail = 0;
             for (uint32_t i = i0; i < i1 && ok; ++i) {
-                const Work w(a, i, lane == 0);
-                const uint32_t half0 = w.tile.kvh * (D / 64);
+                const Work w(a, word, lane == 0);
+                word = Work::fetch(a, i + 1, i1, lane);
+                const uint32_t half0 = w.kvh * (D / 64);
                 for (uint32_t t = 0; t < w.n && ok; ++t) {
-                    const uint32_t first = w.first(t), len = w.length(t);
-                    const uint32_t pages = min(kTilePages, (len - first + kBlock - 1) / kBlock);
-                    const uint32_t* refs = (w.own(t) ? a.suffix_refs + w.list.suf_ref0 : a.prefix_refs + w.list.pre_ref0) +
-                                           first / kBlock;
+                    const uint32_t have = min(kTileTokens, w.length(t) - w.first(t));  // tokens of this tile
+                    const uint32_t pages = (have + kBlock - 1) / kBlock;
                     uint32_t group = 0;
                     if (lane < pages) {
-                        const uint32_t ref = refs[lane] & kRefMask;
+                        const uint32_t ref = w.refs(a, t)[lane] & kRefMask;
                         if (ref >= a.pool_blocks) atomicOr(a.status, DEVERR_REF_RANGE);
                         group = 2 * static_cast<uint32_t>(min(static_cast<uint64_t>(ref), a.pool_blocks));  // past the pool: zeros
                     }
 #pragma unroll
                     for (uint32_t kv = 0; kv < 2; ++kv) {
-                        const uint32_t b = c_full % L::kBufs, round = c_full / L::kBufs;
-                        if (round > 0) ok = warp_wait(&bars.empty[b], (round - 1) & 1, a.status, 50);
-                        if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&bars.full[b], pages * L::kPage);
+                        if (fill > 0 && !(ok = warp_wait(&bars.empty[b], (fill - 1) & 1, a.status, 50))) break;
+                        // V of a partial tile: its rows past the length hold whatever
+                        // the pool or an earlier tile left, and 0 * NaN would reach the
+                        // sums.  It lands on a barrier of its own, is cleared there and
+                        // only then handed over.
+                        const bool tail = kv && have < kTileTokens;
+                        uint64_t* bar = tail ? &bars.tail : &bars.full[b];
+                        if (lane == 0) mbar_arrive_expect_tx(bar, pages * L::kPage);
                         __syncwarp();
                         if (lane < pages)
-                            tma_load_page(smem_u32(bufs + b * L::kBuf + lane * L::kPage), kv ? &tm_v : &tm_k, &bars.full[b],
-                                          half0, group);
-                        ++c_full;
+                            tma_load_page(smem_u32(bufs + b * L::kBuf + lane * L::kPage), kv ? &tm_v : &tm_k, bar, half0, group);
+                        if (tail) {
+                            if (!(ok = warp_wait(&bars.tail, n_tail++ & 1, a.status, 51))) break;
+                            uint8_t* v = bufs + b * L::kBuf;
+#pragma unroll 1
+                            for (uint32_t y = lane; y < (kTileTokens - have) * (D / 8); y += 32) {
+                                const uint32_t row = have + y / (D / 8), ch = y % (D / 8);
+                                *reinterpret_cast<uint4*>(v + (row / 8) * (D * 16) + (ch >> 3) * 1024 + (row & 7) * 128 +
+                                                          (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_proxy_async_shared();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&bars.full[b]);
+                        }
+                        if (++b == L::kBufs) {
+                            b = 0;
+                            ++fill;
+                        }
                     }
                 }
             }
             // every copy has landed before the CTA's shared memory goes (an
             // abandoned wait of the MMA warp may have left some unread)
-            for (uint32_t b = 0; b < L::kBufs && lane == 0; ++b) {
-                if (c_full <= b) break;
-                const uint32_t last = (c_full - 1 - b) / L::kBufs;
-                mbar_drain(&bars.full[b], last & 1);
+            if (lane == 0) {
+                for (uint32_t x = 0; x < L::kBufs; ++x) {
+                    const uint32_t times = fill + (x < b ? 1 : 0);
+                    if (times) mbar_drain(&bars.full[x], (times - 1) & 1);
+                }
+                if (!ok && n_tail) mbar_drain(&bars.tail, (n_tail - 1) & 1);
             }
         } else if (warp == 8) {
-            // ---- MMA
+            // ---- MMA: one thread waits and issues.  Its instructions are what a
+            // step costs besides the products, so indices run along and no lane votes.
+            constexpr uint32_t kQK = f16_idesc(128, kTileTokens, 0), kPV = f16_idesc(128, D, 1);
+            constexpr uint32_t kGroup = D * 16;           // bytes between 8-row groups of a K or V buffer
+            constexpr uint32_t kPairs = L::kBufs / 2;     // K in buffers 0, 2, ..., V in 1, 3, ...
+            constexpr uint32_t kBufStep = L::kBuf >> 4, kQStep = L::kQ >> 4;
+            const uint32_t q_lo = desc_lo(smem_u32(qs), 16), k_lo = desc_lo(smem_u32(bufs), 16),
+                           v_lo = desc_lo(smem_u32(bufs) + L::kBuf, 1024);
+            uint32_t items = i0;
+            Work w(a, word, false);
+            uint32_t kb = 0, kph = 0, vb = 0, vph = 0;  // ring positions of the next K and V tile, their phases
+            uint32_t nq0 = 0, nq1 = 0;                  // QK products so far (half 0, 1)
+            uint32_t np0 = 0, np1 = 0;                  // PV products so far
+            uint32_t ph_q = 0;                          // phases of q_full, a bit per half
             bool ok = true;
-            constexpr uint32_t kQK = f16_idesc(128, 128, 0), kPV = f16_idesc(128, D, 1);
-            constexpr uint32_t kGroup = D * 16;  // bytes between 8-row groups of a K or V buffer
-            uint32_t n_p[2] = {0, 0};            // tiles of each half so far (phase of p_ready, o_done)
-            uint32_t n_q[2] = {0, 0};            // items with tiles for the half so far (phase of q_full)
-            uint32_t base = 0;                   // buffers consumed by earlier items
-            for (uint32_t i = i0; i < i1 && ok; ++i) {
-                const Work w(a, i, false);
-                if (w.n == 0) continue;
-                const uint32_t steps = w.pair ? 2 * w.n : w.n;
-                // Wait for buffer idx; own or prefix tile t's V is cleared from its length on.
-                auto wait_full = [&](uint32_t idx) {
-                    return warp_wait(&bars.full[idx % L::kBufs], (idx / L::kBufs) & 1, a.status, 51);
-                };
-                auto qk = [&](uint32_t h, uint32_t t) {  // S of half h = Q K(t)^T
-                    const uint32_t idx = base + 2 * t;
-                    if (!wait_full(idx)) return false;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t q = smem_u32(qs + h * L::kQ), k = smem_u32(bufs + (idx % L::kBufs) * L::kBuf);
+            while (items < i1) {
+                if (w.n && elect_one()) {
+                    // Products in the order h = 0, 1, 0, 1, ...: step s is token tile s / 2
+                    // of either half's own rows, or tile s of the shared ones.
+                    const uint32_t steps = w.pair ? 2 * w.n : w.n;
+                    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
+                        return mbar_try_wait(bar, parity) || wait_slow(bar, parity, a.status, site);
+                    };
+#pragma unroll 1
+                    for (uint32_t x = 0; x < steps + 4; ++x) {
+                        const uint32_t h = x & 1;
+                        if (x >= 4) {  // O += P V of step x - 4
+                            const uint32_t k = h ? np1++ : np0++;
+                            if (!w.pair || h == 0)
+                                if (!(ok = wait(&bars.full[2 * vb + 1], vph, 51))) break;
+                            if (!(ok = wait(&bars.p_ready[h][k & 1], (k >> 1) & 1, 53))) break;
+                            tc_fence_after();
+                            const uint32_t v = v_lo + 2 * vb * kBufStep, p = tmem + h * 128 + (k & 1) * 64,
+                                           o = tmem + L::kO + h * D;
+                            mma_ts<desc_hi(kGroup)>(o, p, v, kPV, x >= 6);  // the half's first tile of the item starts O
+#pragma unroll
+                            for (uint32_t ks = 1; ks < kTilePages; ++ks)
+                                mma_ts<desc_hi(kGroup)>(o, p + ks * 8, v + ks * (L::kPage >> 4), kPV, 1);
+                            tc_commit(&bars.o_done[h][k & 1]);
+                            if (!w.pair || h == 1) {
+                                tc_commit(&bars.empty[2 * vb + 1]);
+                                if (++vb == kPairs) vb = 0, vph ^= 1;
+                            }
+                        }
+                        // S = Q K^T two tiles ahead: into the S whose P the half's step
+                        // before last has used
+                        const uint32_t s = x < 4 ? x : x - 1, g = s & 1;
+                        if (x == 4 || s >= steps) continue;
+                        const uint32_t k = g ? nq1++ : nq0++;
+                        if (s < 2) {
+                            if (!(ok = wait(&bars.q_full[g], (ph_q >> g) & 1, 52))) break;
+                            ph_q ^= 1u << g;
+                        } else if (s >= 4) {
+                            if (!(ok = wait(&bars.o_done[g][k & 1], ((k - 2) >> 1) & 1, 54))) break;
+                        }
+                        if (!w.pair || g == 0)
+                            if (!(ok = wait(&bars.full[2 * kb], kph, 51))) break;
+                        tc_fence_after();
+                        const uint32_t q = q_lo + g * kQStep, kd = k_lo + 2 * kb * kBufStep, sd = tmem + g * 128 + (k & 1) * 64;
 #pragma unroll
                         for (uint32_t ks = 0; ks < D / 16; ++ks)
-                            mma_ss(tmem + h * 128, sw128_desc(q + (ks / 4) * 16384 + (ks % 4) * 32, 16, 1024),
-                                   sw128_desc(k + (ks / 4) * 1024 + (ks % 4) * 32, 16, kGroup), kQK, ks > 0);
-                        tc_commit(&bars.s_full[h]);
-                        if (!w.pair || h == 1) tc_commit(&bars.empty[idx % L::kBufs]);
-                    }
-                    __syncwarp();
-                    return true;
-                };
-                const uint32_t halves = w.count(1) ? 2 : 1;
-                for (uint32_t h = 0; h < halves && ok; ++h) {
-                    ok = warp_wait(&bars.q_full[h], n_q[h]++ & 1, a.status, 52);
-                    if (ok) ok = qk(h, w.tile_of(0, h));
-                }
-                for (uint32_t st = 0; st < steps && ok; ++st) {
-                    const uint32_t h = st & 1, t = w.pair ? st / 2 : st;
-                    const uint32_t idx = base + 2 * t + 1;
-                    const bool last_use = !w.pair || h == 1;
-                    if (!(ok = wait_full(idx))) break;
-                    if (!w.pair || h == 0) {
-                        // rows past the length hold whatever the pool or an earlier
-                        // tile left: clear them, or 0 * NaN would reach the sums
-                        const uint32_t have = w.length(t) - w.first(t);
-                        if (have < kTileTokens) {
-                            uint8_t* v = bufs + (idx % L::kBufs) * L::kBuf;
-                            for (uint32_t x = lane; x < (kTileTokens - have) * (D / 8); x += 32) {
-                                const uint32_t row = have + x / (D / 8), ch = x % (D / 8);
-                                *reinterpret_cast<uint4*>(v + (row / 8) * kGroup + (ch >> 3) * 1024 + (row & 7) * 128 +
-                                                          (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async_shared();
-                            __syncwarp();
+                            mma_ss<desc_hi(1024), desc_hi(kGroup)>(sd, q + (ks / 4) * 1024 + (ks % 4) * 2,
+                                                                   kd + (ks / 4) * 64 + (ks % 4) * 2, kQK, ks > 0);
+                        tc_commit(&bars.s_full[g][k & 1]);
+                        if (!w.pair || g == 1) {
+                            tc_commit(&bars.empty[2 * kb]);
+                            if (++kb == kPairs) kb = 0, kph ^= 1;
                         }
                     }
-                    if (!(ok = warp_wait(&bars.p_ready[h], n_p[h] & 1, a.status, 53))) break;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t v = smem_u32(bufs + (idx % L::kBufs) * L::kBuf);
-                        const bool more = t >= (w.pair ? 1u : 2u);  // not the half's first tile of the item
-#pragma unroll
-                        for (uint32_t ks = 0; ks < kTilePages; ++ks)
-                            mma_ts(tmem + L::kO + h * D, tmem + h * 128 + ks * 8, sw128_desc(v + ks * L::kPage, 1024, kGroup), kPV,
-                                   more || ks > 0);
-                        tc_commit(&bars.o_done[h]);
-                        if (last_use) tc_commit(&bars.empty[idx % L::kBufs]);
-                    }
-                    __syncwarp();
-                    const uint32_t t_next = w.pair ? t + 1 : t + 2;
-                    if (t_next < w.n) {  // P is read before its columns become the next S
-                        ok = warp_wait(&bars.o_done[h], n_p[h] & 1, a.status, 54);
-                        if (ok) ok = qk(h, t_next);
-                    }
-                    ++n_p[h];
+                    // the last products are done before the next item's S and Q
+                    if (ok && np0) ok = wait(&bars.o_done[0][(np0 - 1) & 1], ((np0 - 1) >> 1) & 1, 55);
+                    if (ok && np1) ok = wait(&bars.o_done[1][(np1 - 1) & 1], ((np1 - 1) >> 1) & 1, 55);
                 }
-                // the last products are done before the next item's S and Q
-                for (uint32_t h = 0; h < halves && ok; ++h)
-                    ok = warp_wait(&bars.o_done[h], (n_p[h] - 1) & 1, a.status, 55);
-                base += 2 * w.n;
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (++items < i1) {
+                    word = Work::fetch(a, items, i1, lane);
+                    w = Work(a, word, false);
+                }
             }
             // nothing in flight when the tensor memory goes (bounded)
-            if (lane == 0) {
+            __syncwarp();
+            if (elect_one()) {
                 tc_commit(&bars.drain);
                 mbar_drain(&bars.drain, 0);
             }
+            __syncwarp();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: half h, one thread per row
         const uint32_t h = warp >> 2, r = tid & 127;
-        const uint32_t lanes = (warp & 3) * 32;  // this warp's tensor-memory lanes
+        const uint32_t lanes = (warp & 3) * 32;  // this warp's rows: tensor-memory lanes
         const uint32_t ts = tmem + (lanes << 16) + h * 128, to = tmem + (lanes << 16) + L::kO + h * D;
+        uint8_t* const qh = qs + h * L::kQ;
         const float scale2 = fabsf(a.scale) * kLog2e;
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale goes into Q
-        uint32_t n_s = 0;                                         // tiles so far (phase of s_full, o_done)
+        constexpr uint32_t kChunks = D / 8, kStep = 32 / kChunks;  // 16-byte chunks of a row; rows per warp-wide copy
+        const uint32_t ch = lane % kChunks, sub = lane / kChunks;
+        uint32_t k = 0;  // tiles so far
         bool ok = true;
         for (uint32_t i = i0; i < i1 && ok; ++i) {
-            const Work w(a, i, false);
+            const Work w(a, word, false);
+            word = Work::fetch(a, i + 1, i1, lane);
             const uint32_t rbase = w.pair ? h * 128 : 0;
             const uint32_t mine = w.rows > rbase ? min(128u, w.rows - rbase) : 0;  // rows of this half
-            const uint32_t g = w.tile.kvh, cnt = w.count(h);
+            const uint32_t cnt = w.count(h);
+            const bool has = r < mine;
+            const bool idle = lanes >= mine;  // no row of this warp
+            uint32_t at = 0;                  // this thread's row of q and out
+            int32_t lim_pre = 0, lim_suf = 0;
+            if (has) {
+                const uint32_t rr = w.row0 + rbase + r, j = rr / a.G;
+                at = a.row_tok[w.tok0 + j] * a.Hq + w.kvh * a.G + (rr - j * a.G);
+                lim_pre = static_cast<int32_t>(w.pre_len);
+                lim_suf = static_cast<int32_t>(w.limit(j));
+            }
             if (cnt) {
-                for (uint32_t x = r; x < 128 * (D / 8); x += 128) {
-                    const uint32_t row = x / (D / 8), ch = x % (D / 8);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (row < mine) {
-                        const uint32_t rr = w.tile.row0 + rbase + row, j = rr / a.G;
-                        const uint64_t at = static_cast<uint64_t>(a.row_tok[w.list.tok0 + j]) * a.Hq + g * a.G + (rr - j * a.G);
-                        v = *reinterpret_cast<const uint4*>(a.q + at * D + ch * 8);
-                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+#pragma unroll 1
+                for (uint32_t y = sub; y < 32; y += kStep) {
+                    const uint64_t row = __shfl_sync(0xffffffffu, at, y);
+                    cp_async16_zfill(qh + (ch >> 3) * 16384 + swz128(lanes + y, ch & 7), a.q + row * D + ch * 8,
+                                     lanes + y < mine);
+                }
+                cp_async_wait_all();
+                if (a.scale < 0.0f) {  // a negative scale goes into Q: each lane flips what it copied
+#pragma unroll 1
+                    for (uint32_t y = sub; y < 32; y += kStep) {
+                        uint4* q = reinterpret_cast<uint4*>(qh + (ch >> 3) * 16384 + swz128(lanes + y, ch & 7));
+                        *q = make_uint4(q->x ^ 0x80008000u, q->y ^ 0x80008000u, q->z ^ 0x80008000u, q->w ^ 0x80008000u);
                     }
-                    *reinterpret_cast<uint4*>(qs + h * L::kQ + (ch >> 3) * 16384 + swz128(row, ch & 7)) = v;
                 }
                 fence_proxy_async_shared();
                 mbar_arrive(&bars.q_full[h]);
             }
-            const bool has = r < mine;
-            const uint32_t rr = w.tile.row0 + rbase + (has ? r : 0), tok = rr / a.G;
-            const int32_t lim_pre = has ? static_cast<int32_t>(w.pre_len) : 0;
-            const int32_t lim_suf = has ? static_cast<int32_t>(suffix_limit(w.list, w.suf_len, tok)) : 0;
-            const bool idle = (warp & 3) * 32 >= mine;  // no row of this warp
             float m = -INFINITY, l = 0.0f;
-            for (uint32_t j = 0; j < cnt; ++j) {
-                const uint32_t t = w.tile_of(j, h);
-                const uint32_t first = w.first(t);
+#pragma unroll 1
+            for (uint32_t j = 0; j < cnt; ++j, ++k) {
+                const uint32_t t = w.tile_of(j, h), first = w.first(t);
                 const int32_t lim = (w.own(t) ? lim_suf : lim_pre) - static_cast<int32_t>(first);
                 // pages of this tile whose reference lies beyond the pool
-                uint32_t bad = 0;
-                {
-                    const uint32_t* refs = (w.own(t) ? a.suffix_refs + w.list.suf_ref0 : a.prefix_refs + w.list.pre_ref0) +
-                                           first / kBlock;
-                    const bool in = lane < kTilePages && first + lane * kBlock < w.length(t);
-                    bad = __ballot_sync(0xffffffffu, in && (refs[in ? lane : 0] & kRefMask) >= a.pool_blocks);
-                }
-                if (!(ok = row_wait(&bars.s_full[h], n_s & 1, a.status, 56))) break;
+                const bool in = lane < kTilePages && first + lane * kBlock < w.length(t);
+                const uint32_t bad =
+                    __ballot_sync(0xffffffffu, in && (w.refs(a, t)[in ? lane : 0] & kRefMask) >= a.pool_blocks);
+                const uint32_t tb = ts + (k & 1) * 64;
+                if (!(ok = row_wait(&bars.s_full[h][k & 1], (k >> 1) & 1, a.status, 56))) break;
                 tc_fence_after();
                 if (!idle) {
-                    uint32_t raw[128];
-                    tc_ld32(ts, raw);
-                    tc_ld32(ts + 32, raw + 32);
-                    tc_ld32(ts + 64, raw + 64);
-                    tc_ld32(ts + 96, raw + 96);
-                    tc_wait_ld();
+                    float v[64];
+                    tc_ld64(tb, v);
                     if (__any_sync(0xffffffffu, lim < static_cast<int32_t>(kTileTokens)) || bad) {
 #pragma unroll
-                        for (int c = 0; c < 128; ++c)
-                            if (c >= lim || ((bad >> (c / 16)) & 1u)) raw[c] = 0xFF800000u;  // -inf
+                        for (int c = 0; c < 64; ++c)
+                            if (c >= lim || ((bad >> (c / 16)) & 1u)) v[c] = -INFINITY;
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(raw[c]));
+                    for (int c = 4; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
                     const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                     const bool grow = m_new > m + kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
@@ -435,91 +539,93 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                             const float f = grow ? ex2(m - to_m) : 1.0f;
                             l *= f;
                             // the previous product has been added before O is rescaled
-                            if (!(ok = row_wait(&bars.o_done[h], (n_s - 1) & 1, a.status, 57))) break;
+                            if (!(ok = row_wait(&bars.o_done[h][(k - 1) & 1], ((k - 1) >> 1) & 1, a.status, 57))) break;
                             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
-                                uint32_t o[32];
+                                float o[32];
                                 tc_ld32(to + c, o);
-                                tc_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                for (int e = 0; e < 32; ++e) o[e] *= f;
                                 tc_st32(to + c, o);
                             }
                         }
                         m = to_m;
                     }
                     const float ms = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float2 sc = make_float2(scale2, scale2), mm = make_float2(-ms, -ms);
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    uint32_t pk[32];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t pk[32];
-#pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const float p0 = ex2(__uint_as_float(raw[half * 64 + c]) * scale2 - ms);
-                            const float p1 = ex2(__uint_as_float(raw[half * 64 + c + 1]) * scale2 - ms);
-                            sum[c & 2] += p0;
-                            sum[(c & 2) + 1] += p1;
-                            const __half2 hp = __floats2half2_rn(p0, p1);
-                            pk[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
-                        }
-                        tc_st32(ts + half * 32, pk);
+                    for (int c = 0; c < 64; c += 2) {
+                        float2 x = fma2(make_float2(v[c], v[c + 1]), sc, mm);
+                        x = make_float2(ex2(x.x), ex2(x.y));
+                        sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], x);
+                        const __half2 hp = __floats2half2_rn(x.x, x.y);
+                        pk[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_st32(tb, pk);
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += sum[0].x + sum[0].y;
                     tc_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_ready[h]);
-                ++n_s;
+                if (lane == 0) mbar_arrive(&bars.p_ready[h][k & 1]);
             }
             if (!ok) break;
             // ---- this half's result
             if (cnt) {
-                if (!(ok = row_wait(&bars.o_done[h], (n_s - 1) & 1, a.status, 58))) break;
+                if (!(ok = row_wait(&bars.o_done[h][(k - 1) & 1], ((k - 1) >> 1) & 1, a.status, 58))) break;
                 tc_fence_after();
             }
-            const bool writes = mine && (w.pair || h == 0 || w.it.two);
-            if (writes && !idle) {
-                float4* po = nullptr;
-                __half* out = nullptr;
-                float inv = 0.0f;
-                if (w.tile.direct) {
-                    inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-                    out = a.out + (static_cast<uint64_t>(a.row_tok[w.list.tok0 + tok]) * a.Hq + g * a.G + (rr - tok * a.G)) * D;
-                } else {
-                    const uint64_t row = w.it.part_row + (w.pair ? rbase : (h ? w.rows : 0u)) + r;
-                    po = reinterpret_cast<float4*>(a.part_o + row * D);
-                    if (has) a.part_ml[row] = make_float2(m * kLn2, l);
-                }
+            if (mine && (w.pair || h == 0 || (w.flags & kTcTwo))) {
+                const bool direct = w.flags & kTcDirect;
+                const float inv = inverse_sum(l);
+                const uint64_t run = w.part_row + (!w.pair && h ? w.rows : 0u);
+                if (!direct && has) a.part_ml[run + rbase + r] = make_float2(m * kLn2, l);
+                if (!idle) {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        if (cnt) {
+                            tc_ld32(to + c, o);
+                        } else {
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    if (cnt) {
-                        tc_ld32(to + c, o);
-                        tc_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0;
-                    }
-                    if (!has) continue;
-                    if (out) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 pack;
-                            __half2* hp = reinterpret_cast<__half2*>(&pack);
-#pragma unroll
-                            for (int y = 0; y < 4; ++y)
-                                hp[y] = __floats2half2_rn(__uint_as_float(o[e + 2 * y]) * inv,
-                                                          __uint_as_float(o[e + 2 * y + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + c + e) = pack;
+                            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                         }
-                    } else {
+                        if (direct) {
+                            // f16 rows into this half's Q (its products are done), copied out row by row below
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            po[(c + e) / 4] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                                                          __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                            for (int e = 0; e < 32; e += 8) {
+                                uint4 pack;
+                                __half2* hp = reinterpret_cast<__half2*>(&pack);
+#pragma unroll
+                                for (int y = 0; y < 4; ++y)
+                                    hp[y] = __floats2half2_rn(o[e + 2 * y] * inv, o[e + 2 * y + 1] * inv);
+                                const uint32_t x = (c + e) / 8;
+                                *reinterpret_cast<uint4*>(qh + (x >> 3) * 16384 + swz128(r, x & 7)) = pack;
+                            }
+                        } else if (has) {
+                            float4* po = reinterpret_cast<float4*>(a.part_o + run * D) + rbase + r;
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                po[static_cast<uint64_t>((c + e) / 4) * w.rows] =
+                                    make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
                     }
+                }
+                if (direct) {
+                    // each warp its own 32 rows: D / 8 lanes write a row's 16-byte chunks
+                    __syncwarp();
+#pragma unroll 2
+                    for (uint32_t y = sub; y < 32; y += kStep) {
+                        const uint64_t row = __shfl_sync(0xffffffffu, at, y);
+                        if (lanes + y < mine)
+                            *reinterpret_cast<uint4*>(a.out + row * D + ch * 8) =
+                                *reinterpret_cast<const uint4*>(qh + (ch >> 3) * 16384 + swz128(lanes + y, ch & 7));
+                    }
+                    __syncwarp();  // the next item's Q goes where the rows were
                 }
             }
             tc_fence_before();  // O and S have been read before the next item's products
