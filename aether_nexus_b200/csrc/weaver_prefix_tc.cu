@@ -24,9 +24,10 @@
 // operand with 8-row groups D * 16 bytes apart, V an MN-major one whose 16
 // tokens per step are one page.
 //
-// Warps 0-3 and 4-7: the halves; warp 8: MMA; warp 9: TMA; warps 10 and 11
-// only complete the third warpgroup, whose registers the first two take over
-// (launched with 168 a thread: 384 * 168 = 64512 >= 256 * 216 + 128 * 64).
+// Warps 0-3 and 4-7: the halves; warp 8: Q K^T; warp 9: TMA; warp 10: P V;
+// warp 11 only completes the third warpgroup, whose registers the first two
+// take over (launched with 168 a thread: 384 * 168 = 64512 >= 256 * 216 + 128 *
+// 64).
 // Code that runs once per item is kept in rolled loops: the first pass over
 // straight-line code is bound by instruction fetch (10 us for an unrolled copy
 // of the query tile).
@@ -66,23 +67,29 @@ struct TcBars {
     // [half][tile of the half & 1]: the products of two tiles of a half may be
     // outstanding, and a parity tells only neighbouring phases apart
     uint64_t q_full[2], s_full[2][2], p_ready[2][2], o_done[2][2];
-    uint64_t tail, drain;
+    uint64_t tail, drain[2];
     uint32_t tmem;
 };
 
-// The bounded wait, by every lane of a warp (same answer in all).  For the MMA
-// and TMA warps the slow path is one function (inlined at every wait it cost
-// their registers); the softmax warps, with a row of S in registers, inline it.
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
+// Bounded waits as in mbar_wait, but the clock is first read after a while:
+// reading %globaltimer takes longer than most of these waits.  For the MMA and
+// TMA warps the slow path is one function (inlined at every wait it cost their
+// registers); the softmax warps, with a row of S in registers, inline it.
+__device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
+    for (uint32_t i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait(bar, parity, status, site);
 }
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
+    return spin(bar, parity, status, site);
+}
+// By every lane of a warp, the same answer in all.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
     const bool ok = mbar_try_wait(bar, parity) || wait_slow(bar, parity, status, site);
     return __all_sync(0xffffffffu, ok);
 }
-
 __device__ __forceinline__ bool row_wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, site));
+    return __all_sync(0xffffffffu, spin(bar, parity, status, site));
 }
 
 // Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 x 128 bytes).
@@ -303,7 +310,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
             }
         }
         mbar_init(&bars.tail, 1);
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.drain[0], 1);
+        mbar_init(&bars.drain[1], 1);
         fence_barrier_init();
     }
     tc_fence_before();
@@ -374,91 +382,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 }
                 if (!ok && n_tail) mbar_drain(&bars.tail, (n_tail - 1) & 1);
             }
-        } else if (warp == 8) {
-            // ---- MMA: one thread waits and issues.  Its instructions are what a
-            // step costs besides the products, so indices run along and no lane votes.
+        } else if (warp == 8 || warp == 10) {
+            // ---- the products: warp 8 issues S = Q K^T, warp 10 O += P V, one
+            // thread each.  A step of one thread that did both took 1200 clocks,
+            // 80 to 100 for every barrier polled or committed to, against 670 of
+            // the products themselves.
             constexpr uint32_t kQK = f16_idesc(128, kTileTokens, 0), kPV = f16_idesc(128, D, 1);
-            constexpr uint32_t kGroup = D * 16;           // bytes between 8-row groups of a K or V buffer
-            constexpr uint32_t kPairs = L::kBufs / 2;     // K in buffers 0, 2, ..., V in 1, 3, ...
+            constexpr uint32_t kGroup = D * 16;        // bytes between 8-row groups of a K or V buffer
+            constexpr uint32_t kPairs = L::kBufs / 2;  // K in buffers 0, 2, ..., V in 1, 3, ...
             constexpr uint32_t kBufStep = L::kBuf >> 4, kQStep = L::kQ >> 4;
+            const bool is_qk = warp == 8;
             const uint32_t q_lo = desc_lo(smem_u32(qs), 16), k_lo = desc_lo(smem_u32(bufs), 16),
                            v_lo = desc_lo(smem_u32(bufs) + L::kBuf, 1024);
-            uint32_t items = i0;
-            Work w(a, word, false);
-            uint32_t kb = 0, kph = 0, vb = 0, vph = 0;  // ring positions of the next K and V tile, their phases
-            uint32_t nq0 = 0, nq1 = 0;                  // QK products so far (half 0, 1)
-            uint32_t np0 = 0, np1 = 0;                  // PV products so far
-            uint32_t ph_q = 0;                          // phases of q_full, a bit per half
+            uint32_t b = 0, ph = 0;         // ring position of the next K (V) tile, its phase
+            uint32_t n0 = 0, n1 = 0;        // tiles of either half so far
+            uint32_t ph_q = 0;              // phases of q_full, a bit per half
             bool ok = true;
-            while (items < i1) {
-                if (w.n && elect_one()) {
-                    // Products in the order h = 0, 1, 0, 1, ...: step s is token tile s / 2
-                    // of either half's own rows, or tile s of the shared ones.
-                    const uint32_t steps = w.pair ? 2 * w.n : w.n;
-                    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
-                        return mbar_try_wait(bar, parity) || wait_slow(bar, parity, a.status, site);
-                    };
+            auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
+                return mbar_try_wait(bar, parity) || wait_slow(bar, parity, a.status, site);
+            };
+            for (uint32_t i = i0; i < i1; ++i) {
+                const Work w(a, word, false);
+                word = Work::fetch(a, i + 1, i1, lane);
+                // In the order h = 0, 1, 0, 1, ...: step s is token tile s / 2 of either
+                // half's own rows, or tile s of the shared ones.
+                const uint32_t steps = w.pair ? 2 * w.n : w.n;
+                if (elect_one()) {
+                    if (is_qk) {
 #pragma unroll 1
-                    for (uint32_t x = 0; x < steps + 4; ++x) {
-                        const uint32_t h = x & 1;
-                        if (x >= 4) {  // O += P V of step x - 4
-                            const uint32_t k = h ? np1++ : np0++;
+                        for (uint32_t s = 0; s < steps; ++s) {
+                            const uint32_t h = s & 1, k = h ? n1++ : n0++;
+                            if (s < 2) {
+                                if (!(ok = wait(&bars.q_full[h], (ph_q >> h) & 1, 52))) break;
+                                ph_q ^= 1u << h;
+                            }
                             if (!w.pair || h == 0)
-                                if (!(ok = wait(&bars.full[2 * vb + 1], vph, 51))) break;
+                                if (!(ok = wait(&bars.full[2 * b], ph, 51))) break;
+                            // the S whose P the half's step before last has used
+                            if (k >= 2 && !(ok = wait(&bars.o_done[h][k & 1], ((k - 2) >> 1) & 1, 54))) break;
+                            tc_fence_after();
+                            const uint32_t q = q_lo + h * kQStep, kd = k_lo + 2 * b * kBufStep, sd = tmem + h * 128 + (k & 1) * 64;
+#pragma unroll
+                            for (uint32_t ks = 0; ks < D / 16; ++ks)
+                                mma_ss<desc_hi(1024), desc_hi(kGroup)>(sd, q + (ks / 4) * 1024 + (ks % 4) * 2,
+                                                                       kd + (ks / 4) * 64 + (ks % 4) * 2, kQK, ks > 0);
+                            tc_commit(&bars.s_full[h][k & 1]);
+                            if (!w.pair || h == 1) {
+                                tc_commit(&bars.empty[2 * b]);
+                                if (++b == kPairs) b = 0, ph ^= 1;
+                            }
+                        }
+                    } else {
+#pragma unroll 1
+                        for (uint32_t s = 0; s < steps; ++s) {
+                            const uint32_t h = s & 1, k = h ? n1++ : n0++;
+                            if (!w.pair || h == 0)
+                                if (!(ok = wait(&bars.full[2 * b + 1], ph, 51))) break;
                             if (!(ok = wait(&bars.p_ready[h][k & 1], (k >> 1) & 1, 53))) break;
                             tc_fence_after();
-                            const uint32_t v = v_lo + 2 * vb * kBufStep, p = tmem + h * 128 + (k & 1) * 64,
-                                           o = tmem + L::kO + h * D;
-                            mma_ts<desc_hi(kGroup)>(o, p, v, kPV, x >= 6);  // the half's first tile of the item starts O
+                            const uint32_t v = v_lo + 2 * b * kBufStep, p = tmem + h * 128 + (k & 1) * 64, o = tmem + L::kO + h * D;
+                            mma_ts<desc_hi(kGroup)>(o, p, v, kPV, s >= 2);  // the half's first tile of the item starts O
 #pragma unroll
                             for (uint32_t ks = 1; ks < kTilePages; ++ks)
                                 mma_ts<desc_hi(kGroup)>(o, p + ks * 8, v + ks * (L::kPage >> 4), kPV, 1);
                             tc_commit(&bars.o_done[h][k & 1]);
                             if (!w.pair || h == 1) {
-                                tc_commit(&bars.empty[2 * vb + 1]);
-                                if (++vb == kPairs) vb = 0, vph ^= 1;
+                                tc_commit(&bars.empty[2 * b + 1]);
+                                if (++b == kPairs) b = 0, ph ^= 1;
                             }
                         }
-                        // S = Q K^T two tiles ahead: into the S whose P the half's step
-                        // before last has used
-                        const uint32_t s = x < 4 ? x : x - 1, g = s & 1;
-                        if (x == 4 || s >= steps) continue;
-                        const uint32_t k = g ? nq1++ : nq0++;
-                        if (s < 2) {
-                            if (!(ok = wait(&bars.q_full[g], (ph_q >> g) & 1, 52))) break;
-                            ph_q ^= 1u << g;
-                        } else if (s >= 4) {
-                            if (!(ok = wait(&bars.o_done[g][k & 1], ((k - 2) >> 1) & 1, 54))) break;
-                        }
-                        if (!w.pair || g == 0)
-                            if (!(ok = wait(&bars.full[2 * kb], kph, 51))) break;
-                        tc_fence_after();
-                        const uint32_t q = q_lo + g * kQStep, kd = k_lo + 2 * kb * kBufStep, sd = tmem + g * 128 + (k & 1) * 64;
-#pragma unroll
-                        for (uint32_t ks = 0; ks < D / 16; ++ks)
-                            mma_ss<desc_hi(1024), desc_hi(kGroup)>(sd, q + (ks / 4) * 1024 + (ks % 4) * 2,
-                                                                   kd + (ks / 4) * 64 + (ks % 4) * 2, kQK, ks > 0);
-                        tc_commit(&bars.s_full[g][k & 1]);
-                        if (!w.pair || g == 1) {
-                            tc_commit(&bars.empty[2 * kb]);
-                            if (++kb == kPairs) kb = 0, kph ^= 1;
-                        }
                     }
-                    // the last products are done before the next item's S and Q
-                    if (ok && np0) ok = wait(&bars.o_done[0][(np0 - 1) & 1], ((np0 - 1) >> 1) & 1, 55);
-                    if (ok && np1) ok = wait(&bars.o_done[1][(np1 - 1) & 1], ((np1 - 1) >> 1) & 1, 55);
                 }
                 if (!__all_sync(0xffffffffu, ok)) break;
-                if (++items < i1) {
-                    word = Work::fetch(a, items, i1, lane);
-                    w = Work(a, word, false);
-                }
             }
             // nothing in flight when the tensor memory goes (bounded)
             __syncwarp();
             if (elect_one()) {
-                tc_commit(&bars.drain);
-                mbar_drain(&bars.drain, 0);
+                tc_commit(&bars.drain[is_qk]);
+                mbar_drain(&bars.drain[is_qk], 0);
             }
             __syncwarp();
         }
