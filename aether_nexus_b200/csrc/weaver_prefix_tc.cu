@@ -200,6 +200,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -427,10 +433,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                                 mma_ss<desc_hi(1024), desc_hi(kGroup)>(sd, q + (ks / 4) * 1024 + (ks % 4) * 2,
                                                                        kd + (ks / 4) * 64 + (ks % 4) * 2, kQK, ks > 0);
                             tc_commit(&bars.s_full[h][k & 1]);
-                            if (!w.pair || h == 1) {
-                                tc_commit(&bars.empty[2 * b]);
-                                if (++b == kPairs) b = 0, ph ^= 1;
-                            }
+                            if ((!w.pair || h == 1) && ++b == kPairs) b = 0, ph ^= 1;
                         }
                     } else {
 #pragma unroll 1
@@ -440,6 +443,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                                 if (!(ok = wait(&bars.full[2 * b + 1], ph, 51))) break;
                             if (!(ok = wait(&bars.p_ready[h][k & 1], (k >> 1) & 1, 53))) break;
                             tc_fence_after();
+                            // P of the tile's last half: its Q K^T is done, and K with it (an
+                            // arrive takes a fifth of a commit's time)
+                            if (!w.pair || h == 1) mbar_arrive(&bars.empty[2 * b]);
                             const uint32_t v = v_lo + 2 * b * kBufStep, p = tmem + h * 128 + (k & 1) * 64, o = tmem + L::kO + h * D;
                             mma_ts<desc_hi(kGroup)>(o, p, v, kPV, s >= 2);  // the half's first tile of the item starts O
 #pragma unroll
@@ -510,14 +516,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 mbar_arrive(&bars.q_full[h]);
             }
             float m = -INFINITY, l = 0.0f;
+            // a tile's limit and this lane's page reference, a tile ahead
+            int32_t lim = 0;
+            uint32_t ref = 0;
+            auto look = [&](uint32_t j) {
+                const uint32_t t = w.tile_of(j, h), first = w.first(t);
+                lim = (w.own(t) ? lim_suf : lim_pre) - static_cast<int32_t>(first);
+                ref = 0;
+                if (j < cnt && lane < kTilePages && first + lane * kBlock < w.length(t)) ref = w.refs(a, t)[lane] & kRefMask;
+            };
+            look(0);
 #pragma unroll 1
             for (uint32_t j = 0; j < cnt; ++j, ++k) {
-                const uint32_t t = w.tile_of(j, h), first = w.first(t);
-                const int32_t lim = (w.own(t) ? lim_suf : lim_pre) - static_cast<int32_t>(first);
                 // pages of this tile whose reference lies beyond the pool
-                const bool in = lane < kTilePages && first + lane * kBlock < w.length(t);
-                const uint32_t bad =
-                    __ballot_sync(0xffffffffu, in && (w.refs(a, t)[in ? lane : 0] & kRefMask) >= a.pool_blocks);
+                const uint32_t bad = __ballot_sync(0xffffffffu, ref >= a.pool_blocks);
                 const uint32_t tb = ts + (k & 1) * 64;
                 if (!(ok = row_wait(&bars.s_full[h][k & 1], (k >> 1) & 1, a.status, 56))) break;
                 tc_fence_after();
@@ -531,8 +543,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                     }
                     float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int c = 4; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
-                    const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                    for (int c = 4; c < 60; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[c + e], v[c + 4 + e]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], v[60 + e]);
+                    const float m_new = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale2;
                     const bool grow = m_new > m + kRescale;
                     if (__any_sync(0xffffffffu, grow)) {
                         const float to_m = grow ? m_new : m;
@@ -553,6 +569,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                         }
                         m = to_m;
                     }
+                    look(j + 1);
                     const float ms = m == -INFINITY ? 0.0f : m;
                     const float2 sc = make_float2(scale2, scale2), mm = make_float2(-ms, -ms);
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
