@@ -24,10 +24,9 @@
 // operand with 8-row groups D * 16 bytes apart, V an MN-major one whose 16
 // tokens per step are one page.
 //
-// Warps 0-3 and 4-7: the halves; warp 8: Q K^T; warp 9: TMA; warp 10: P V;
-// warp 11 only completes the third warpgroup, whose registers the first two
-// take over (launched with 168 a thread: 384 * 168 = 64512 >= 256 * 216 + 128 *
-// 64).
+// Warps 0-3 and 4-7: the halves; warp 8: Q K^T; warp 10: P V; warps 9 and 11:
+// TMA of K and of V.  The first two warpgroups take over registers of the third
+// (launched with 168 a thread: 384 * 168 = 64512 >= 256 * 216 + 128 * 64).
 // Code that runs once per item is kept in rolled loops: the first pass over
 // straight-line code is bound by instruction fetch (10 us for an unrolled copy
 // of the query tile).
@@ -82,6 +81,16 @@ __device__ __forceinline__ bool spin(uint64_t* bar, uint32_t parity, uint32_t* s
 }
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
     return spin(bar, parity, status, site);
+}
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 // By every lane of a warp, the same answer in all.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
@@ -328,63 +337,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 9) {
-            // ---- TMA: K and V of every token tile, in turn, into the ring
+        if (warp == 9 || warp == 11) {
+            // ---- TMA: warp 9 brings K, warp 11 V of every token tile into their half
+            // of the ring (buffers 0, 2, ... and 1, 3, ...).  The page references of
+            // the next tile are loaded ahead and the copies issued by one thread with
+            // uniform operands: one warp that did both, loading as it went, took 1400
+            // clocks a tile and bounded the kernel.
+            const uint32_t kv = warp == 11;
+            const CUtensorMap* map = kv ? &tm_v : &tm_k;
+            constexpr uint32_t kPairs = L::kBufs / 2;
             bool ok = true;
-            uint32_t b = 0, fill = 0;  // next buffer; how often the ring has been filled
+            uint32_t b = 0, fill = 0;  // next buffer pair; how often the ring has been filled
             uint32_t n_tail = 0;
             for (uint32_t i = i0; i < i1 && ok; ++i) {
-                const Work w(a, word, lane == 0);
+                const Work w(a, word, lane == 0 && !kv);
                 word = Work::fetch(a, i + 1, i1, lane);
                 const uint32_t half0 = w.kvh * (D / 64);
+                auto reference = [&](uint32_t t) {
+                    return t < w.n && lane < kTilePages && w.first(t) + lane * kBlock < w.length(t) ? w.refs(a, t)[lane] & kRefMask : 0u;
+                };
+                uint32_t next = reference(0);
                 for (uint32_t t = 0; t < w.n && ok; ++t) {
+                    const uint32_t ref = next;
+                    next = reference(t + 1);
                     const uint32_t have = min(kTileTokens, w.length(t) - w.first(t));  // tokens of this tile
                     const uint32_t pages = (have + kBlock - 1) / kBlock;
-                    uint32_t group = 0;
-                    if (lane < pages) {
-                        const uint32_t ref = w.refs(a, t)[lane] & kRefMask;
-                        if (ref >= a.pool_blocks) atomicOr(a.status, DEVERR_REF_RANGE);
-                        group = 2 * static_cast<uint32_t>(min(static_cast<uint64_t>(ref), a.pool_blocks));  // past the pool: zeros
-                    }
+                    if (ref >= a.pool_blocks && !kv) atomicOr(a.status, DEVERR_REF_RANGE);
+                    const uint32_t group = 2 * static_cast<uint32_t>(min(static_cast<uint64_t>(ref), a.pool_blocks));  // past the pool: zeros
+                    if (fill > 0 && !(ok = warp_wait(&bars.empty[2 * b + kv], (fill - 1) & 1, a.status, 50))) break;
+                    // V of a partial tile: its rows past the length hold whatever the
+                    // pool or an earlier tile left, and 0 * NaN would reach the sums.
+                    // It lands on a barrier of its own, is cleared there and only then
+                    // handed over.
+                    const bool tail = kv && have < kTileTokens;
+                    uint64_t* bar = tail ? &bars.tail : &bars.full[2 * b + kv];
+                    uint8_t* buf = bufs + (2 * b + kv) * L::kBuf;
+                    uint32_t at[kTilePages];
 #pragma unroll
-                    for (uint32_t kv = 0; kv < 2; ++kv) {
-                        if (fill > 0 && !(ok = warp_wait(&bars.empty[b], (fill - 1) & 1, a.status, 50))) break;
-                        // V of a partial tile: its rows past the length hold whatever
-                        // the pool or an earlier tile left, and 0 * NaN would reach the
-                        // sums.  It lands on a barrier of its own, is cleared there and
-                        // only then handed over.
-                        const bool tail = kv && have < kTileTokens;
-                        uint64_t* bar = tail ? &bars.tail : &bars.full[b];
-                        if (lane == 0) mbar_arrive_expect_tx(bar, pages * L::kPage);
-                        __syncwarp();
-                        if (lane < pages)
-                            tma_load_page(smem_u32(bufs + b * L::kBuf + lane * L::kPage), kv ? &tm_v : &tm_k, bar, half0, group);
-                        if (tail) {
-                            if (!(ok = warp_wait(&bars.tail, n_tail++ & 1, a.status, 51))) break;
-                            uint8_t* v = bufs + b * L::kBuf;
+                    for (uint32_t p = 0; p < kTilePages; ++p) at[p] = __shfl_sync(0xffffffffu, group, p);
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar, pages * L::kPage);
+#pragma unroll
+                        for (uint32_t p = 0; p < kTilePages; ++p)
+                            if (p < pages) tma_load_page(smem_u32(buf + p * L::kPage), map, bar, half0, at[p]);
+                    }
+                    __syncwarp();
+                    if (tail) {
+                        if (!(ok = warp_wait(&bars.tail, n_tail++ & 1, a.status, 51))) break;
 #pragma unroll 1
-                            for (uint32_t y = lane; y < (kTileTokens - have) * (D / 8); y += 32) {
-                                const uint32_t row = have + y / (D / 8), ch = y % (D / 8);
-                                *reinterpret_cast<uint4*>(v + (row / 8) * (D * 16) + (ch >> 3) * 1024 + (row & 7) * 128 +
-                                                          (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async_shared();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&bars.full[b]);
+                        for (uint32_t y = lane; y < (kTileTokens - have) * (D / 8); y += 32) {
+                            const uint32_t row = have + y / (D / 8), ch = y % (D / 8);
+                            *reinterpret_cast<uint4*>(buf + (row / 8) * (D * 16) + (ch >> 3) * 1024 + (row & 7) * 128 +
+                                                      (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
-                        if (++b == L::kBufs) {
-                            b = 0;
-                            ++fill;
-                        }
+                        fence_proxy_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars.full[2 * b + kv]);
+                    }
+                    if (++b == kPairs) {
+                        b = 0;
+                        ++fill;
                     }
                 }
             }
             // every copy has landed before the CTA's shared memory goes (an
-            // abandoned wait of the MMA warp may have left some unread)
+            // abandoned wait of the MMA warps may have left some unread)
             if (lane == 0) {
-                for (uint32_t x = 0; x < L::kBufs; ++x) {
+                for (uint32_t x = 0; x < kPairs; ++x) {
                     const uint32_t times = fill + (x < b ? 1 : 0);
-                    if (times) mbar_drain(&bars.full[x], (times - 1) & 1);
+                    if (times) mbar_drain(&bars.full[2 * x + kv], (times - 1) & 1);
                 }
                 if (!ok && n_tail) mbar_drain(&bars.tail, (n_tail - 1) & 1);
             }
@@ -516,7 +537,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 mbar_arrive(&bars.q_full[h]);
             }
             float m = -INFINITY, l = 0.0f;
-            // a tile's limit and this lane's page reference, a tile ahead
+            // a tile's limit, its pages beyond the pool, and whether any row of the
+            // warp needs the mask: a tile ahead, among the exponentials
             int32_t lim = 0;
             uint32_t ref = 0;
             auto look = [&](uint32_t j) {
@@ -525,18 +547,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 ref = 0;
                 if (j < cnt && lane < kTilePages && first + lane * kBlock < w.length(t)) ref = w.refs(a, t)[lane] & kRefMask;
             };
+            auto masked_pages = [&](uint32_t& bad) {
+                bad = __ballot_sync(0xffffffffu, ref >= a.pool_blocks);
+                return __any_sync(0xffffffffu, lim < static_cast<int32_t>(kTileTokens)) || bad;
+            };
             look(0);
+            uint32_t bad;
+            bool masked = masked_pages(bad), ready = false;
 #pragma unroll 1
             for (uint32_t j = 0; j < cnt; ++j, ++k) {
-                // pages of this tile whose reference lies beyond the pool
-                const uint32_t bad = __ballot_sync(0xffffffffu, ref >= a.pool_blocks);
                 const uint32_t tb = ts + (k & 1) * 64;
-                if (!(ok = row_wait(&bars.s_full[h][k & 1], (k >> 1) & 1, a.status, 56))) break;
+                if (!ready && !(ok = row_wait(&bars.s_full[h][k & 1], (k >> 1) & 1, a.status, 56))) break;
                 tc_fence_after();
                 if (!idle) {
                     float v[64];
                     tc_ld64(tb, v);
-                    if (__any_sync(0xffffffffu, lim < static_cast<int32_t>(kTileTokens)) || bad) {
+                    if (masked) {
 #pragma unroll
                         for (int c = 0; c < 64; ++c)
                             if (c >= lim || ((bad >> (c / 16)) & 1u)) v[c] = -INFINITY;
@@ -582,14 +608,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                         const __half2 hp = __floats2half2_rn(x.x, x.y);
                         pk[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
+                    // the next S is usually there by now; a poll takes 170 clocks
+                    const bool next = mbar_test(&bars.s_full[h][(k + 1) & 1], ((k + 1) >> 1) & 1);
                     tc_st32(tb, pk);
                     sum[0] = add2(sum[0], sum[1]);
                     l += sum[0].x + sum[0].y;
                     tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.p_ready[h][k & 1]);
+                    masked = masked_pages(bad);
+                    ready = __all_sync(0xffffffffu, next);
+                } else if (lane == 0) {
+                    mbar_arrive(&bars.p_ready[h][k & 1]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_ready[h][k & 1]);
             }
             if (!ok) break;
             // ---- this half's result
