@@ -10,9 +10,10 @@
 //   O += P V (P from tensor memory, V in shared memory)
 // A tile of more than 128 rows gives each half 128 rows of it and both take
 // every token tile; a smaller one gives both halves the same rows and every
-// other token tile.  m is the row's maximum up to 2^8: the accumulator is
-// rescaled only when the maximum has grown by more than that, since p <= 2^8
-// and its f16 rounding is relative.
+// other token tile.  m is the row's maximum up to 2^15: the accumulator is
+// rescaled only when the maximum has grown by more than that, since p <= 2^15
+// is well inside f16, whose rounding is relative (at 2^8 a tile in ten of
+// normal data still stopped a half for 900 clocks).
 //
 // Tensor memory (512 columns): two S of either half (64 columns each; P lies
 // in the first 32), O of either half (D each).  With two S the product for the
@@ -49,7 +50,7 @@ constexpr uint32_t kTilePages = kTcPages;
 constexpr uint32_t kTileTokens = kTilePages * kBlock;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRescale = 8.0f;  // log2 of the growth of the maximum that forces a rescale
+constexpr float kRescale = 15.0f;  // log2 of the growth of the maximum that forces a rescale: p stays below f16's 2^16
 
 template <int D>
 struct TcLayout {
@@ -279,7 +280,6 @@ struct Work {
     __device__ __forceinline__ uint32_t limit(uint32_t j) const { return suffix_limit(flags & kTcCausal, suf_len, ntok, j); }
     // token tiles of half h
     __device__ __forceinline__ uint32_t count(uint32_t h) const { return pair ? n : (n + 1 - h) / 2; }
-    __device__ __forceinline__ uint32_t tile_of(uint32_t j, uint32_t h) const { return pair ? j : 2 * j + h; }
     // token tile t: whether of the own pages, its first token there, tokens of the list, its first page reference
     __device__ __forceinline__ bool own(uint32_t t) const { return t >= n_pre; }
     __device__ __forceinline__ uint32_t first(uint32_t t) const {
@@ -537,32 +537,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 mbar_arrive(&bars.q_full[h]);
             }
             float m = -INFINITY, l = 0.0f;
-            // a tile's limit, its pages beyond the pool, and whether any row of the
-            // warp needs the mask: a tile ahead, among the exponentials
-            int32_t lim = 0;
-            uint32_t ref = 0;
-            auto look = [&](uint32_t j) {
-                const uint32_t t = w.tile_of(j, h), first = w.first(t);
-                lim = (w.own(t) ? lim_suf : lim_pre) - static_cast<int32_t>(first);
-                ref = 0;
-                if (j < cnt && lane < kTilePages && first + lane * kBlock < w.length(t)) ref = w.refs(a, t)[lane] & kRefMask;
+            // Pages beyond the pool: looked for once per item (a look at every tile
+            // took 130 clocks of it), and tile by tile only where there are any.
+            bool any_bad = false;
+#pragma unroll 1
+            for (uint32_t t = 0; t < w.n; t += 32 / kTilePages) {
+                const uint32_t tl = t + lane / kTilePages, pg = lane % kTilePages;
+                const bool in = tl < w.n && w.first(tl) + pg * kBlock < w.length(tl);
+                any_bad |= __any_sync(0xffffffffu, in && (w.refs(a, tl)[in ? pg : 0] & kRefMask) >= a.pool_blocks);
+            }
+            // Tokens of the tile that this row sees, and that the warp's first row sees:
+            // the rows' limits rise with the row, so the first one says whether any row
+            // needs the mask.  They fall by a tile's tokens from tile to tile.
+            const uint32_t step = w.pair ? 1 : 2;
+            uint32_t t = w.pair ? 0 : h;
+            int32_t lim = 0, low = 0;
+            auto enter = [&] {  // tile t is the half's first of a list
+                const int32_t first = static_cast<int32_t>(w.first(t));
+                lim = (w.own(t) ? lim_suf : lim_pre) - first;
+                low = __shfl_sync(0xffffffffu, lim, 0);
             };
-            auto masked_pages = [&](uint32_t& bad) {
-                bad = __ballot_sync(0xffffffffu, ref >= a.pool_blocks);
-                return __any_sync(0xffffffffu, lim < static_cast<int32_t>(kTileTokens)) || bad;
-            };
-            look(0);
-            uint32_t bad;
-            bool masked = masked_pages(bad), ready = false;
+            enter();
+            bool ready = false;
 #pragma unroll 1
             for (uint32_t j = 0; j < cnt; ++j, ++k) {
                 const uint32_t tb = ts + (k & 1) * 64;
                 if (!ready && !(ok = row_wait(&bars.s_full[h][k & 1], (k >> 1) & 1, a.status, 56))) break;
                 tc_fence_after();
+                uint32_t bad = 0;
+                if (any_bad) {
+                    const bool in = lane < kTilePages && w.first(t) + lane * kBlock < w.length(t);
+                    bad = __ballot_sync(0xffffffffu, in && (w.refs(a, t)[in ? lane : 0] & kRefMask) >= a.pool_blocks);
+                }
                 if (!idle) {
                     float v[64];
                     tc_ld64(tb, v);
-                    if (masked) {
+                    if (low < static_cast<int32_t>(kTileTokens) || bad) {
 #pragma unroll
                         for (int c = 0; c < 64; ++c)
                             if (c >= lim || ((bad >> (c / 16)) & 1u)) v[c] = -INFINITY;
@@ -595,7 +605,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                         }
                         m = to_m;
                     }
-                    look(j + 1);
                     const float ms = m == -INFINITY ? 0.0f : m;
                     const float2 sc = make_float2(scale2, scale2), mm = make_float2(-ms, -ms);
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -608,20 +617,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                         const __half2 hp = __floats2half2_rn(x.x, x.y);
                         pk[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
-                    // the next S is usually there by now; a poll takes 170 clocks
-                    const bool next = mbar_test(&bars.s_full[h][(k + 1) & 1], ((k + 1) >> 1) & 1);
                     tc_st32(tb, pk);
+                    // the next S is usually there by now; a poll takes 170 clocks, here beside
+                    // the store (before the store, which then waits for it, it cost a tenth)
+                    const bool next = mbar_test(&bars.s_full[h][(k + 1) & 1], ((k + 1) >> 1) & 1);
                     sum[0] = add2(sum[0], sum[1]);
                     l += sum[0].x + sum[0].y;
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_ready[h][k & 1]);
-                    masked = masked_pages(bad);
                     ready = __all_sync(0xffffffffu, next);
                 } else if (lane == 0) {
                     mbar_arrive(&bars.p_ready[h][k & 1]);
                 }
+                t += step;
+                lim -= static_cast<int32_t>(step * kTileTokens);
+                low -= static_cast<int32_t>(step * kTileTokens);
+                if (t >= w.n_pre && t < w.n_pre + step) enter();
             }
             if (!ok) break;
             // ---- this half's result
