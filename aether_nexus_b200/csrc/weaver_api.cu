@@ -1975,7 +1975,7 @@ struct weaver_prefix_plan {
     weaver_prefix_shape shape{};
     PrefixArgs base{};
     void* arena = nullptr;
-    uint32_t n_items16 = 0, n_tc_ctas = 0;
+    uint32_t n_items16 = 0, n_tc_ctas = 0, max_slots = 0;
     uint64_t n_prefix_pages = 0, n_suffix_pages = 0;
     cudaStream_t last_stream = nullptr;
 };
@@ -2073,10 +2073,8 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
         return o;
     };
     const uint32_t zero[2] = {0, 0};
-    const size_t o_lists = place(t.lists.data(), t.lists.size() * sizeof(PrefixList)),
-                 o_tiles = place(t.tiles.data(), t.tiles.size() * sizeof(PrefixTile)),
-                 o_items = place(t.items16.data(), t.items16.size() * sizeof(PrefixItem)),
-                 o_tc = place(t.items_tc.data(), t.items_tc.size() * sizeof(PrefixTcItem)),
+    const size_t o_items = place(t.items16.data(), t.items16.size() * sizeof(PrefixItem)),
+                 o_tc = place(t.items_tc.data(), t.items_tc.size() * sizeof(PrefixItem)),
                  o_ptr = place(t.tc_ptr.data(), t.tc_ptr.size() * 4), o_row = place(t.row_tok.data(), t.row_tok.size() * 4),
                  o_merge = place(t.merge_rows.data(), t.merge_rows.size() * sizeof(PrefixMergeRow)),
                  o_status = place(zero, sizeof(zero));
@@ -2093,14 +2091,13 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     }
     plan->shape = *sh;
     plan->n_items16 = static_cast<uint32_t>(t.items16.size());
+    plan->max_slots = t.max_slots;
     plan->n_tc_ctas = static_cast<uint32_t>(t.tc_ptr.size()) - 1;
     plan->n_prefix_pages = prefix_indptr[NG];
     plan->n_suffix_pages = suffix_indptr[B];
     PrefixArgs& a = plan->base;
-    a.lists = reinterpret_cast<const PrefixList*>(base + o_lists);
-    a.tiles = reinterpret_cast<const PrefixTile*>(base + o_tiles);
     a.items = reinterpret_cast<const PrefixItem*>(base + o_items);
-    a.tc_items = reinterpret_cast<const PrefixTcItem*>(base + o_tc);
+    a.tc_items = reinterpret_cast<const PrefixItem*>(base + o_tc);
     a.tc_ptr = reinterpret_cast<const uint32_t*>(base + o_ptr);
     a.row_tok = reinterpret_cast<const uint32_t*>(base + o_row);
     a.merge_rows = reinterpret_cast<const PrefixMergeRow*>(base + o_merge);
@@ -2173,15 +2170,15 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
     plan->last_stream = s;
     DeviceScope dev(plan->device);
     WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
+    if (plan->n_items16) WEAVER_CUDA_TRY(launch_prefix_rows16(a, plan->n_items16, s), "prefix attention launch");
     if (plan->n_tc_ctas) {
         CUtensorMap tm_k, tm_v;
         int rc;
         if ((rc = encode_pages(&tm_k, v->hot_k, v->hot_pool_blocks, a.Hkv, a.D, "hot_k"))) return rc;
         if ((rc = encode_pages(&tm_v, v->hot_v, v->hot_pool_blocks, a.Hkv, a.D, "hot_v"))) return rc;
-        WEAVER_CUDA_TRY(launch_prefix_tc(a, tm_k, tm_v, plan->n_tc_ctas, s), "prefix attention launch");
+        WEAVER_CUDA_TRY(launch_prefix_tc(a, tm_k, tm_v, plan->n_tc_ctas, plan->n_items16 > 0, s), "prefix attention launch");
     }
-    if (plan->n_items16) WEAVER_CUDA_TRY(launch_prefix_rows16(a, plan->n_items16, s), "prefix attention launch");
-    if (a.n_merge) WEAVER_CUDA_TRY(launch_prefix_merge(a, s), "prefix merge launch");
+    if (a.n_merge) WEAVER_CUDA_TRY(launch_prefix_merge(a, plan->max_slots, s), "prefix merge launch");
     return WEAVER_OK;
 }
 

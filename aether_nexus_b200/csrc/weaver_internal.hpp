@@ -360,32 +360,30 @@ struct PrefixTile {
     uint32_t list, kvh, row0, rows;
     uint32_t n_slots, direct;  // direct: its only item writes the output
 };
-// Pages blk0 .. blk1-1 of a 16-row tile's list, counted over the prefix's pages
-// and then the own ones.
+// An item: pages (16-row tiles) or token tiles of kTcPages pages (tensor-memory
+// tiles) t0 .. t1-1 of a tile's list, the prefix's pre_units first and then the
+// own pages', with all that a kernel needs of the tile and the list: read by
+// one warp-wide load.
 struct PrefixItem {
     uint64_t part_row;
-    uint32_t tile, blk0, blk1, pad;
-};
-// Token tiles t0 .. t1-1 (kTcPages pages each) of a tensor-memory tile's list (the prefix's
-// pre_tiles, then the own pages'), with all that the kernel needs of the tile
-// and the list: read by one warp-wide load.
-struct PrefixTcItem {
-    uint64_t part_row;
     uint32_t tok0, row0, rows, kvh, ntok;
-    uint32_t pre_ref0, pre_blocks, pre_len, pre_tiles;
+    uint32_t pre_ref0, pre_blocks, pre_len, pre_units;
     uint32_t suf_ref0, suf_blocks, suf_len;
     uint32_t t0, t1;
-    uint32_t flags;  // kTcCausal, kTcTwo, kTcDirect
+    uint32_t flags;  // kPxCausal, kPxDirect, kPxTwo
     uint32_t pad[3];
 };
-constexpr uint32_t kTcPages = 4;  // pages of a token tile: 64 tokens
-constexpr uint32_t kTcCausal = 1, kTcDirect = 2;
-constexpr uint32_t kTcTwo = 4;  // at most 128 rows and several token tiles: the two halves of the CTA write a slot each
-static_assert(sizeof(PrefixTcItem) == 80, "one word per lane of a warp");
-// One output row to be merged from its rows of up to two tiles (~0: none).
+constexpr uint32_t kPxCausal = 1, kPxDirect = 2;
+constexpr uint32_t kPxTwo = 4;  // at most 128 rows and several token tiles: the two halves of the CTA write a slot each
+static_assert(sizeof(PrefixItem) == 80, "one word per lane of a warp");
+// One output row to be merged: row row[s] of n[s] runs of step[s] rows each from
+// row run0[s] of the partials, of up to two tiles.
 struct PrefixMergeRow {
-    uint32_t out_row, tile[2], row[2];
+    uint64_t run0[2];
+    uint32_t step[2], n[2], row[2];
+    uint32_t out_row, pad;
 };
+constexpr uint32_t kTcPages = 4;  // pages of a token tile: 64 tokens
 struct PrefixArgs {
     const __half *q, *k, *v;
     __half* out;
@@ -394,10 +392,8 @@ struct PrefixArgs {
     const uint32_t *prefix_lens, *suffix_lens;  // null: every page is full
     uint64_t pool_blocks;
     const PrefixItem* items;           // of the 16-row tiles
-    const PrefixTcItem* tc_items;      // of the tensor-memory tiles, CTA c's are [tc_ptr[c], tc_ptr[c+1])
+    const PrefixItem* tc_items;      // of the tensor-memory tiles, CTA c's are [tc_ptr[c], tc_ptr[c+1])
     const uint32_t* tc_ptr;
-    const PrefixTile* tiles;
-    const PrefixList* lists;
     const uint32_t* row_tok;
     const PrefixMergeRow* merge_rows;
     float2* part_ml;
@@ -415,18 +411,20 @@ struct PrefixGeometry {
 struct PrefixTables {
     std::vector<PrefixList> lists;
     std::vector<PrefixTile> tiles;
-    std::vector<PrefixItem> items16;
-    std::vector<PrefixTcItem> items_tc;
+    std::vector<PrefixItem> items16, items_tc;
     std::vector<uint32_t> tc_ptr, row_tok;
     std::vector<PrefixMergeRow> merge_rows;
     uint64_t part_rows = 0;
+    uint32_t max_slots = 0;  // of a merged row
 };
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t);
+// The kernels of one run, in this order, each but the first a programmatic
+// dependent launch (after = true) of the one before.
 cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s);
-cudaError_t launch_prefix_merge(const PrefixArgs& a, cudaStream_t s);
+cudaError_t launch_prefix_merge(const PrefixArgs& a, uint32_t max_slots, cudaStream_t s);
 // Tiles of up to 256 rows on tcgen05 (tm_k / tm_v: the pools as [blocks * 2][8
 // rows][Hkv * D / 64][64], boxes of one page of one head, 128-byte swizzle).
 cudaError_t launch_prefix_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas,
-                             cudaStream_t s);
+                             bool after, cudaStream_t s);
 
 }  // namespace weaver

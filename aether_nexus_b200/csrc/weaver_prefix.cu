@@ -50,13 +50,13 @@ struct PxLayout {
 };
 
 template <int D>
-__device__ __forceinline__ void px_issue(uint8_t* st, const PrefixArgs& a, uint64_t block, bool ok, uint32_t pos0,
-                                         uint32_t len, uint32_t g, uint32_t lane) {
+__device__ __forceinline__ void px_issue(uint8_t* st, const PrefixArgs& a, uint64_t block, uint32_t pos0, uint32_t len,
+                                         uint32_t g, uint32_t lane) {
     constexpr uint32_t kChunks = D / 8;
 #pragma unroll
     for (uint32_t i = lane; i < 16 * kChunks; i += 32) {
         const uint32_t row = i / kChunks, ch = i % kChunks;
-        const bool valid = ok && pos0 + row < len;
+        const bool valid = pos0 + row < len;
         const uint64_t off = valid ? ((block * kBlock + row) * a.Hkv + g) * D + ch * 8 : 0ull;
         const uint32_t so = (ch >> 3) * FaTile<D>::kBox + swz128(row, ch & 7);
         cp_async16_zfill(st + so, a.k + off, valid);
@@ -65,51 +65,52 @@ __device__ __forceinline__ void px_issue(uint8_t* st, const PrefixArgs& a, uint6
 }
 
 template <int D>
-__global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixArgs a) {
+__global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const __grid_constant__ PrefixArgs a) {
     using L = PxLayout<D>;
     constexpr int KS = D / 16, NT = D / 8;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __half* qs = reinterpret_cast<__half*>(smem + (L::kRing > L::kRed ? L::kRing : L::kRed));
     float* red = reinterpret_cast<float*>(smem);
+    launch_dependents();
 
+    // Three latencies before the pages are under way: the item, then the lengths,
+    // page references and tokens that it names, then query rows and pages.
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2;
-    const PrefixItem it = a.items[blockIdx.x];
-    const PrefixTile tile = a.tiles[it.tile];
-    const PrefixList list = a.lists[tile.list];
-    const uint32_t g = tile.kvh, rows = tile.rows;
-    const uint32_t pre_len = page_len(a.prefix_lens, list.pre_len, list.pre_blocks, a.status, tid == 0);
-    const uint32_t suf_len = page_len(a.suffix_lens, list.suf_len, list.suf_blocks, a.status, tid == 0);
-    auto out_row = [&](uint32_t r) {  // row r of the tile in q and out
-        const uint32_t rr = tile.row0 + r, j = rr / a.G;
-        return static_cast<uint64_t>(a.row_tok[list.tok0 + j]) * a.Hq + g * a.G + (rr - j * a.G);
+    const uint32_t word = lane < sizeof(PrefixItem) / 4 ? reinterpret_cast<const uint32_t*>(a.items + blockIdx.x)[lane] : 0u;
+    auto field = [&](uint32_t w) { return __shfl_sync(0xffffffffu, word, w); };
+    const uint64_t part_row = static_cast<uint64_t>(field(1)) << 32 | field(0);
+    const uint32_t tok0 = field(2), row0 = field(3), rows = field(4), g = field(5), ntok = field(6);
+    const uint32_t pre_ref0 = field(7), pre_blocks = field(8), pre_i = field(9), suf_ref0 = field(11), suf_blocks = field(12),
+                   suf_i = field(13), t0 = field(14), t1 = field(15), flags = field(16);
+    const uint32_t pre_len = page_len(a.prefix_lens, pre_i, pre_blocks, a.status, tid == 0);
+    const uint32_t suf_len = page_len(a.suffix_lens, suf_i, suf_blocks, a.status, tid == 0);
+    // this warp's pages are t0 + warp, + 4, ...: lane i holds the reference of the i-th of 32
+    auto reference = [&](uint32_t k0) {
+        const uint32_t p = t0 + warp + 4 * (k0 + lane);
+        return p >= t1 ? 0u : (p < pre_blocks ? a.prefix_refs[pre_ref0 + p] : a.suffix_refs[suf_ref0 + p - pre_blocks]) & kRefMask;
     };
-
+    uint32_t ref = reference(0);
+    uint32_t at = 0;  // lane r: row r of the tile in q and out
+    if (lane < rows) {
+        const uint32_t rr = row0 + lane, j = rr / a.G;
+        at = a.row_tok[tok0 + j] * a.Hq + g * a.G + (rr - j * a.G);
+    }
     for (uint32_t i = tid; i < 16 * (D / 8); i += kPxThreads) {
         const uint32_t r = i / (D / 8), ch = i % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows) v = *reinterpret_cast<const uint4*>(a.q + out_row(r) * D + ch * 8);
-        *reinterpret_cast<uint4*>(qs + r * D + ch * 8) = v;
+        const uint64_t row = __shfl_sync(0xffffffffu, at, r);
+        cp_async16_zfill(qs + r * D + ch * 8, a.q + row * D + ch * 8, r < rows);
     }
-    __syncthreads();
-    uint32_t qf[KS][4];
-    fa_load_q<D>(qs, qf, lane);
+    cp_async_commit();
+    const bool causal = flags & kPxCausal;
     int32_t lim_pre[2], lim_suf[2];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
         const uint32_t r = gid + 8 * hh;
         lim_pre[hh] = r < rows ? static_cast<int32_t>(pre_len) : 0;
-        lim_suf[hh] = r < rows ? static_cast<int32_t>(suffix_limit(list.causal, suf_len, list.ntok, (tile.row0 + r) / a.G)) : 0;
+        lim_suf[hh] = r < rows ? static_cast<int32_t>(suffix_limit(causal, suf_len, ntok, (row0 + r) / a.G)) : 0;
     }
-    // the item's pages below the lengths and the tile's largest limit: n_pre of
-    // the prefix from blk0, then own ones from suf0; this warp takes every fourth
-    const uint32_t top = suffix_limit(list.causal, suf_len, list.ntok, (tile.row0 + rows - 1) / a.G);
-    const uint32_t p1 = min(it.blk1, (pre_len + kBlock - 1) / kBlock);
-    const uint32_t n_pre = p1 > it.blk0 ? p1 - it.blk0 : 0;
-    const uint32_t suf0 = it.blk0 > list.pre_blocks ? it.blk0 - list.pre_blocks : 0;
-    const uint32_t s1 = min(it.blk1 > list.pre_blocks ? it.blk1 - list.pre_blocks : 0, (top + kBlock - 1) / kBlock);
-    const uint32_t n = n_pre + (s1 > suf0 ? s1 - suf0 : 0);
-    const uint32_t nb = warp < n ? (n - warp + 3) / 4 : 0;
+    const uint32_t top = suffix_limit(causal, suf_len, ntok, (row0 + rows - 1) / a.G);  // the largest of the tile
 
     uint8_t* ring = smem + warp * L::kWarpRing;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
@@ -119,29 +120,49 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
 
-    uint32_t valid = 0;  // bit k & 1: page k's reference is in the pool
-    auto own = [&](uint32_t k) { return warp + 4 * k >= n_pre; };
-    auto page = [&](uint32_t k) { return own(k) ? suf0 + (warp + 4 * k - n_pre) : it.blk0 + warp + 4 * k; };
-    auto issue = [&](uint32_t k) {
-        const uint32_t b = page(k);
-        const uint32_t ref = (own(k) ? a.suffix_refs[list.suf_ref0 + b] : a.prefix_refs[list.pre_ref0 + b]) & kRefMask;
+    uint32_t qf[KS][4];
+    bool have_q = false;
+    for (uint32_t k0 = 0; t0 + warp + 4 * k0 < t1; k0 += 32) {
+        if (k0) ref = reference(k0);
+        // the pages with tokens that some row sees
+        const uint32_t p = t0 + warp + 4 * (k0 + lane);
+        const bool own = p >= pre_blocks;
+        const uint32_t pos = (own ? p - pre_blocks : p) * kBlock;
+        const bool in = p < t1 && pos < (own ? top : pre_len);
         const bool ok = ref < a.pool_blocks;
-        if (!ok && lane == 0) atomicOr(a.status, DEVERR_REF_RANGE);
-        valid = (valid & ~(1u << (k & 1))) | (ok ? 1u << (k & 1) : 0u);
-        px_issue<D>(ring + (k & 1) * L::kStage, a, ref, ok, b * kBlock, own(k) ? suf_len : pre_len, g, lane);
-    };
-    if (nb > 0) issue(0);
-    cp_async_commit();
-    for (uint32_t k = 0; k < nb; ++k) {
-        const bool ok = (valid >> (k & 1)) & 1u;
-        if (k + 1 < nb) issue(k + 1);
+        if (in && !ok) atomicOr(a.status, DEVERR_REF_RANGE);
+        uint32_t todo = __ballot_sync(0xffffffffu, in && ok), next = todo;  // pages to compute, to fetch
+        uint32_t stage = 0, fetched = 0;
+        auto issue = [&] {
+            const uint32_t i = __ffs(next) - 1;
+            next &= next - 1;
+            px_issue<D>(ring + (fetched++ & 1) * L::kStage, a, __shfl_sync(0xffffffffu, ref, i), __shfl_sync(0xffffffffu, pos, i),
+                        __shfl_sync(0xffffffffu, own, i) ? suf_len : pre_len, g, lane);
+        };
+        if (next) issue();
         cp_async_commit();
-        cp_async_wait1();  // page k has landed (this lane's copies)
-        __syncwarp();      // ... and every lane's
-        const uint8_t* Ks = ring + (k & 1) * L::kStage;
-        fa_block<D>(Ks, Ks + L::kTile, qf, own(k) ? lim_suf : lim_pre, static_cast<int32_t>(page(k) * kBlock), a.scale, ok,
-                    m_run, l_run, o, lane);
-        __syncwarp();  // every lane done with the stage before it is refilled
+        while (todo) {
+            const uint32_t i = __ffs(todo) - 1;
+            todo &= todo - 1;
+            if (next) issue();
+            cp_async_commit();
+            cp_async_wait1();  // the page (and the query rows) have landed, this lane's copies
+            if (!have_q) {
+                named_bar(1, kPxThreads);  // ... and every thread's
+                fa_load_q<D>(qs, qf, lane);
+                have_q = true;
+            }
+            __syncwarp();
+            const uint8_t* Ks = ring + (stage++ & 1) * L::kStage;
+            const bool o_own = __shfl_sync(0xffffffffu, own, i);
+            fa_block<D>(Ks, Ks + L::kTile, qf, o_own ? lim_suf : lim_pre,
+                        static_cast<int32_t>(__shfl_sync(0xffffffffu, pos, i)), a.scale, true, m_run, l_run, o, lane);
+            __syncwarp();  // every lane done with the stage before it is refilled
+        }
+    }
+    if (!have_q) {  // a warp without pages keeps the others' appointment
+        cp_async_wait_all();
+        named_bar(1, kPxThreads);
     }
     cp_async_wait_all();
     __syncthreads();  // the rings are dead: reuse the space for the warps' partials
@@ -162,44 +183,68 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const PrefixA
             Lsum += pw[1] * f;
             O += pw[2 + d] * f;
         }
-        if (tile.direct) {
-            a.out[out_row(r) * D + d] = __float2half_rn(O * inverse_sum(Lsum));
+        if (flags & kPxDirect) {
+            const uint32_t rr = row0 + r, j = rr / a.G;
+            const uint64_t row = static_cast<uint64_t>(a.row_tok[tok0 + j]) * a.Hq + g * a.G + (rr - j * a.G);
+            a.out[row * D + d] = __float2half_rn(O * inverse_sum(Lsum));
         } else {
-            if (d == 0) a.part_ml[it.part_row + r] = make_float2(M, Lsum);
-            a.part_o[it.part_row * D + (d / 4 * rows + r) * 4 + d % 4] = O;
+            if (d == 0) a.part_ml[part_row + r] = make_float2(M, Lsum);
+            a.part_o[part_row * D + (d / 4 * rows + r) * 4 + d % 4] = O;
         }
     }
 }
 
-// A thread per (merged row, four dimensions), rows fastest: one pass over the
-// slots of the row's tiles with the running maximum.
-template <int D>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
-    constexpr uint32_t kRows = 8;  // neighbouring rows per run of D / 4 threads each
-    const uint64_t idx = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const uint64_t i = idx / (kRows * D / 4) * kRows + idx % kRows;
-    const uint32_t c = static_cast<uint32_t>(idx / kRows % (D / 4));
-    if (i >= a.n_merge) return;
-    const PrefixMergeRow mr = a.merge_rows[i];
+// A thread per (merged row, four dimensions, share of the row's runs), rows
+// fastest: one pass over the runs with the running maximum, then the kShares
+// threads of a row and dimensions join theirs in shared memory.  Few rows
+// behind a long prefix have a run per CTA that attended to it, and one thread
+// would walk through them a latency at a time.
+template <int D, uint32_t kShares>
+__global__ void __launch_bounds__(8 * D / 4) prefix_merge_kernel(const __grid_constant__ PrefixArgs a) {
+    constexpr uint32_t kRows = 8 / kShares;  // neighbouring rows per CTA of 8 * D / 4 threads
+    __shared__ float sm[kShares > 1 ? kShares : 1][kRows][D / 4][6];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t r = tid % kRows, c = tid / kRows % (D / 4), share = tid / (kRows * D / 4);
+    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRows + r;
+    const bool in = i < a.n_merge;
+    const PrefixMergeRow mr = a.merge_rows[in ? i : 0];
+    wait_prerequisites();
     float M = -INFINITY, L = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto join = [&](float m, float l, float4 y) {
+        const float Mn = fmaxf(M, m);
+        const float f0 = exp_shift(M, Mn), f1 = exp_shift(m, Mn);
+        M = Mn;
+        L = L * f0 + l * f1;
+        O = make_float4(O.x * f0 + y.x * f1, O.y * f0 + y.y * f1, O.z * f0 + y.z * f1, O.w * f0 + y.w * f1);
+    };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        if (mr.tile[s] == ~0u) continue;
-        const PrefixTile T = a.tiles[mr.tile[s]];
-        const float2* ml = a.part_ml + T.part_row0 + mr.row[s];
-        const float4* o = reinterpret_cast<const float4*>(a.part_o + T.part_row0 * D) + c * T.rows + mr.row[s];
+        // row `row` of runs that start at rows run0, run0 + step, ...
+        const uint64_t step = mr.step[s], run0 = mr.run0[s];
+        const uint32_t row = mr.row[s];
+        const uint32_t n = in ? mr.n[s] : 0u;
 #pragma unroll 4
-        for (uint32_t k = 0; k < T.n_slots; ++k) {
-            const float2 x = ml[static_cast<uint64_t>(k) * T.rows];
-            const float4 y = o[static_cast<uint64_t>(k) * T.rows * (D / 4)];
-            const float Mn = fmaxf(M, x.x);
-            const float f0 = exp_shift(M, Mn), f1 = exp_shift(x.x, Mn);
-            M = Mn;
-            L = L * f0 + x.y * f1;
-            O = make_float4(O.x * f0 + y.x * f1, O.y * f0 + y.y * f1, O.z * f0 + y.z * f1, O.w * f0 + y.w * f1);
+        for (uint32_t k = share; k < n; k += kShares) {
+            const float2 x = a.part_ml[run0 + k * step + row];
+            const float4 y = reinterpret_cast<const float4*>(a.part_o + (run0 + k * step) * D)[c * step + row];
+            join(x.x, x.y, y);
         }
     }
+    if (kShares > 1) {
+        float* mine = sm[share][r][c];
+        mine[0] = M, mine[1] = L, mine[2] = O.x, mine[3] = O.y, mine[4] = O.z, mine[5] = O.w;
+        __syncthreads();
+        if (share) return;
+        M = -INFINITY, L = 0.0f;
+        O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t k = 0; k < kShares; ++k) {
+            const float* x = sm[k][r][c];
+            join(x[0], x[1], make_float4(x[2], x[3], x[4], x[5]));
+        }
+    }
+    if (!in) return;
     const uint64_t row = mr.out_row;
     if (a.out_m) {
         if (c == 0) {
@@ -325,6 +370,17 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     }
     uint64_t part_rows = 0;
 
+    auto item_of = [&](const PrefixTile& T, uint32_t unit) {
+        const PrefixList& L = t->lists[T.list];
+        PrefixItem it{};
+        it.tok0 = L.tok0, it.row0 = T.row0, it.rows = T.rows, it.kvh = T.kvh, it.ntok = L.ntok;
+        it.pre_ref0 = L.pre_ref0, it.pre_blocks = L.pre_blocks, it.pre_len = L.pre_len;
+        it.pre_units = (L.pre_blocks + unit - 1) / unit;
+        it.suf_ref0 = L.suf_ref0, it.suf_blocks = L.suf_blocks, it.suf_len = L.suf_len;
+        it.flags = L.causal ? kPxCausal : 0;
+        return it;
+    };
+
     // 16-row tiles: about three CTAs fit an SM; items of whole multiples of
     // four pages (one per warp), as long as that still gives two full waves
     const uint64_t target = 6ull * n_sm;
@@ -337,11 +393,11 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         T.direct = T.n_slots == 1 && !joined[T.list];
         T.part_row0 = part_rows;
         for (uint32_t s = 0; s < T.n_slots; ++s) {
-            PrefixItem it{};
-            it.tile = ti;
-            it.blk0 = static_cast<uint32_t>(s * per);
-            it.blk1 = static_cast<uint32_t>(std::min<uint64_t>(n, (s + 1) * per));
+            PrefixItem it = item_of(T, 1);
             it.part_row = part_rows + s * rows;
+            it.t0 = static_cast<uint32_t>(s * per);
+            it.t1 = static_cast<uint32_t>(std::min<uint64_t>(n, (s + 1) * per));
+            it.flags |= T.direct ? kPxDirect : 0;
             t->items16.push_back(it);
         }
         if (!T.direct) part_rows += T.n_slots * rows;
@@ -355,7 +411,6 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     uint32_t cta = 0;
     for (const TcTile& x : tc) {
         PrefixTile& T = t->tiles[x.tile];
-        const PrefixList& L = t->lists[T.list];
         const size_t first = t->items_tc.size();
         T.part_row0 = part_rows;
         spent += kItemCost;
@@ -370,16 +425,12 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
                 continue;
             }
             take = std::min<uint64_t>(take, x.n - b);
-            PrefixTcItem it{};
+            PrefixItem it = item_of(T, kTcPages);
             it.part_row = part_rows + static_cast<uint64_t>(T.n_slots) * T.rows;
-            it.tok0 = L.tok0, it.row0 = T.row0, it.rows = T.rows, it.kvh = T.kvh, it.ntok = L.ntok;
-            it.pre_ref0 = L.pre_ref0, it.pre_blocks = L.pre_blocks, it.pre_len = L.pre_len;
-            it.pre_tiles = (L.pre_blocks + kTcPages - 1) / kTcPages;
-            it.suf_ref0 = L.suf_ref0, it.suf_blocks = L.suf_blocks, it.suf_len = L.suf_len;
             it.t0 = b;
             it.t1 = static_cast<uint32_t>(b + take);
             const bool two = T.rows <= 128 && take > 1;
-            it.flags = (L.causal ? kTcCausal : 0) | (two ? kTcTwo : 0);
+            it.flags |= two ? kPxTwo : 0;
             T.n_slots += two ? 2 : 1;
             t->items_tc.push_back(it);
             b += static_cast<uint32_t>(take);
@@ -387,7 +438,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         }
         T.direct = T.n_slots == 1 && !joined[T.list];
         if (T.direct)
-            t->items_tc[first].flags |= kTcDirect;
+            t->items_tc[first].flags |= kPxDirect;
         else
             part_rows += static_cast<uint64_t>(T.n_slots) * T.rows;
     }
@@ -398,17 +449,22 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     // (their zeros) included
     for (uint32_t q = 0; q < geo.q_indptr[B]; ++q)
         for (uint32_t h = 0; h < geo.Hq; ++h) {
-            PrefixMergeRow m{q * geo.Hq + h, {none, none}, {0, 0}};
+            PrefixMergeRow m{};
+            m.out_row = q * geo.Hq + h;
             const uint32_t list[2] = {at[q].x, at[q].z}, tok[2] = {at[q].y, at[q].w};
             bool direct = false;
             for (int s = 0; s < 2; ++s) {
                 if (list[s] == none || !pages(list[s])) continue;
                 const PrefixList& L = t->lists[list[s]];
                 const uint32_t r = tok[s] * G + h % G;
-                m.tile[s] = L.tile0 + h / G * L.n_tiles + r / L.tile_rows;
+                const PrefixTile& T = t->tiles[L.tile0 + h / G * L.n_tiles + r / L.tile_rows];
+                m.run0[s] = T.part_row0;
+                m.step[s] = T.rows;
+                m.n[s] = T.n_slots;
                 m.row[s] = r % L.tile_rows;
-                direct |= t->tiles[m.tile[s]].direct != 0;
+                direct |= T.direct != 0;
             }
+            if (!direct) t->max_slots = std::max(t->max_slots, m.n[0] + m.n[1]);
             if (!direct) t->merge_rows.push_back(m);
         }
 }
@@ -425,19 +481,22 @@ cudaError_t rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <int D, uint32_t kShares>
+cudaError_t merge(const PrefixArgs& a, cudaStream_t s) {
+    constexpr uint32_t kRows = 8 / kShares;
+    return launch_pdl(prefix_merge_kernel<D, kShares>, dim3((a.n_merge + kRows - 1) / kRows), dim3(8 * D / 4), 0, true, s, a);
+}
+
 }  // namespace
 
 cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s) {
     return a.D == 128 ? rows16<128>(a, n_items, s) : rows16<64>(a, n_items, s);
 }
 
-cudaError_t launch_prefix_merge(const PrefixArgs& a, cudaStream_t s) {
-    const uint32_t grid = static_cast<uint32_t>((a.n_merge + 7ull) / 8 * 8 * (a.D / 4) / 256) + 1;
-    if (a.D == 128)
-        prefix_merge_kernel<128><<<grid, 256, 0, s>>>(a);
-    else
-        prefix_merge_kernel<64><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_prefix_merge(const PrefixArgs& a, uint32_t max_slots, cudaStream_t s) {
+    // four shares of the runs where a row has more than eight
+    if (max_slots > 8) return a.D == 128 ? merge<128, 4>(a, s) : merge<64, 4>(a, s);
+    return a.D == 128 ? merge<128, 1>(a, s) : merge<64, 1>(a, s);
 }
 
 }  // namespace weaver

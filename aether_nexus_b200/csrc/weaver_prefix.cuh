@@ -24,6 +24,26 @@ __device__ __forceinline__ uint32_t suffix_limit(bool causal, uint32_t len, uint
     return lim > 0 ? static_cast<uint32_t>(lim) : 0u;
 }
 
+// Programmatic dependent launch: let the next kernel of the stream start / wait
+// until the one before has completed and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, bool after, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // 1 / l; 0 for a row that saw nothing; NaN stays NaN.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); }
 

@@ -254,7 +254,7 @@ struct Work {
 
     // This lane's word of item i's record.
     static __device__ __forceinline__ uint32_t fetch(const PrefixArgs& a, uint32_t i, uint32_t end, uint32_t lane) {
-        return i < end && lane < sizeof(PrefixTcItem) / 4 ? reinterpret_cast<const uint32_t*>(a.tc_items + i)[lane] : 0u;
+        return i < end && lane < sizeof(PrefixItem) / 4 ? reinterpret_cast<const uint32_t*>(a.tc_items + i)[lane] : 0u;
     }
     __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t word, bool report) {
         auto at = [&](uint32_t w) { return __shfl_sync(0xffffffffu, word, w); };
@@ -277,7 +277,7 @@ struct Work {
         const uint32_t s1 = min(t1 > cap ? t1 - cap : 0, (top + kTileTokens - 1) / kTileTokens);
         n = n_pre + (s1 > suf0 ? s1 - suf0 : 0);
     }
-    __device__ __forceinline__ uint32_t limit(uint32_t j) const { return suffix_limit(flags & kTcCausal, suf_len, ntok, j); }
+    __device__ __forceinline__ uint32_t limit(uint32_t j) const { return suffix_limit(flags & kPxCausal, suf_len, ntok, j); }
     // token tiles of half h
     __device__ __forceinline__ uint32_t count(uint32_t h) const { return pair ? n : (n + 1 - h) / 2; }
     // token tile t: whether of the own pages, its first token there, tokens of the list, its first page reference
@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t i0 = a.tc_ptr[blockIdx.x], i1 = a.tc_ptr[blockIdx.x + 1];
+    launch_dependents();
 
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
@@ -642,8 +643,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 if (!(ok = row_wait(&bars.o_done[h][(k - 1) & 1], ((k - 1) >> 1) & 1, a.status, 58))) break;
                 tc_fence_after();
             }
-            if (mine && (w.pair || h == 0 || (w.flags & kTcTwo))) {
-                const bool direct = w.flags & kTcDirect;
+            if (mine && (w.pair || h == 0 || (w.flags & kPxTwo))) {
+                const bool direct = w.flags & kPxDirect;
                 const float inv = inverse_sum(l);
                 const uint64_t run = w.part_row + (!w.pair && h ? w.rows : 0u);
                 if (!direct && has) a.part_ml[run + rbase + r] = make_float2(m * kLn2, l);
@@ -694,6 +695,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
             tc_fence_before();  // O and S have been read before the next item's products
         }
     }
+    // the 16-row tiles' kernel has completed when this one has, for the merge
+    if (tid == 0) wait_prerequisites();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -701,20 +704,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
 }
 
 template <int D>
-cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas, cudaStream_t s) {
+cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas, bool after,
+                      cudaStream_t s) {
     const size_t smem = 1024 + TcLayout<D>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    prefix_tc_kernel<D><<<n_ctas, kTcThreads, smem, s>>>(tm_k, tm_v, a);
-    return cudaGetLastError();
+    return launch_pdl(prefix_tc_kernel<D>, dim3(n_ctas), dim3(kTcThreads), smem, after, s, tm_k, tm_v, a);
 }
 
 }  // namespace
 
-cudaError_t launch_prefix_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas,
+cudaError_t launch_prefix_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas, bool after,
                              cudaStream_t s) {
-    return a.D == 128 ? launch_tc<128>(a, tm_k, tm_v, n_ctas, s) : launch_tc<64>(a, tm_k, tm_v, n_ctas, s);
+    return a.D == 128 ? launch_tc<128>(a, tm_k, tm_v, n_ctas, after, s) : launch_tc<64>(a, tm_k, tm_v, n_ctas, after, s);
 }
 
 }  // namespace weaver
