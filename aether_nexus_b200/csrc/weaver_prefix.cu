@@ -168,28 +168,40 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const __grid_
     __syncthreads();  // the rings are dead: reuse the space for the warps' partials
     fa_store_partial<D>(red + warp * 16 * (D + 2), m_run, l_run, o, lane);
     __syncthreads();
-    for (uint32_t x = tid; x < 16 * D; x += kPxThreads) {
-        // four dimensions of a row to each quad of threads, the next row to the next quad
-        const uint32_t r = (x / 4) % 16, d = x / 64 * 4 + x % 4;
-        if (r >= rows) continue;
-        float M = -INFINITY;
+    // each row's maximum and sum over the four warps, and the warps' factors
+    if (tid < 16) {
+        float M = -INFINITY, Lsum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, red[(w * 16 + r) * (D + 2)]);
-        float Lsum = 0.0f, O = 0.0f;
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, red[(w * 16 + tid) * (D + 2)]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float* pw = red + (w * 16 + tid) * (D + 2);
+            const float f = exp_shift(pw[0], M);
+            Lsum += pw[1] * f;
+            pw[0] = f;
+        }
+        red[tid * (D + 2) + 1] = inverse_sum(Lsum);
+        if (!(flags & kPxDirect) && tid < rows) a.part_ml[part_row + tid] = make_float2(M, Lsum);
+    }
+    __syncthreads();
+    // four dimensions of a row per thread, the next row to the next thread
+    for (uint32_t x = tid; x < rows * (D / 4); x += kPxThreads) {
+        const uint32_t r = x % rows, c = x / rows;
+        float O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float* pw = red + (w * 16 + r) * (D + 2);
-            const float f = exp_shift(pw[0], M);
-            Lsum += pw[1] * f;
-            O += pw[2 + d] * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] += pw[2 + c * 4 + e] * pw[0];
         }
         if (flags & kPxDirect) {
+            const float inv = red[r * (D + 2) + 1];
             const uint32_t rr = row0 + r, j = rr / a.G;
             const uint64_t row = static_cast<uint64_t>(a.row_tok[tok0 + j]) * a.Hq + g * a.G + (rr - j * a.G);
-            a.out[row * D + d] = __float2half_rn(O * inverse_sum(Lsum));
+            __half2 h[2] = {__floats2half2_rn(O[0] * inv, O[1] * inv), __floats2half2_rn(O[2] * inv, O[3] * inv)};
+            *reinterpret_cast<uint2*>(a.out + row * D + c * 4) = *reinterpret_cast<const uint2*>(h);
         } else {
-            if (d == 0) a.part_ml[part_row + r] = make_float2(M, Lsum);
-            a.part_o[part_row * D + (d / 4 * rows + r) * 4 + d % 4] = O;
+            *reinterpret_cast<float4*>(a.part_o + part_row * D + x * 4ull) = make_float4(O[0], O[1], O[2], O[3]);
         }
     }
 }
