@@ -334,7 +334,7 @@ struct RopeArgs {
     uint64_t pool_rows;
     uint32_t T, Hq, Hkv, D, rot;
     uint32_t bf16, interleaved;
-    uint32_t tokens_per_cta;           // set by the launcher
+    uint32_t warps_per_token;          // set by the launcher
     float eps, amplitude;
     uint64_t freq[64];
 };
