@@ -170,12 +170,13 @@ SIGNATURES = [
                                      c_void_p]),
     ("weaver_rope_create", c_int, [c_void_p, ctypes.POINTER(RopeConfigC), ctypes.POINTER(c_void_p)]),
     ("weaver_rope_destroy", None, [c_void_p]),
-    ("weaver_rope_rotate", c_int, [c_void_p, ctypes.POINTER(RopeViewsC), c_void_p]),
-    ("weaver_rope_append", c_int, [c_void_p, ctypes.POINTER(RopeViewsC), c_void_p]),
+    # (the views as a struct or as its bytes)
+    ("weaver_rope_rotate", c_int, [c_void_p, c_void_p, c_void_p]),
+    ("weaver_rope_append", c_int, [c_void_p, c_void_p, c_void_p]),
     ("weaver_prefix_plan_create", c_int, [c_void_p, ctypes.POINTER(PrefixShapeC), c_void_p, c_void_p, c_void_p,
                                           c_void_p, ctypes.POINTER(c_void_p)]),
     ("weaver_prefix_plan_destroy", None, [c_void_p]),
-    ("weaver_prefix_run", c_int, [c_void_p, ctypes.POINTER(PrefixViewsC), c_void_p]),
+    ("weaver_prefix_run", c_int, [c_void_p, c_void_p, c_void_p]),
     ("weaver_prefix_plan_kernel_count", c_int, [c_void_p]),
     ("weaver_prefix_plan_status", c_int, [c_void_p]),
 ]

@@ -1867,13 +1867,16 @@ int encode_pages(CUtensorMap* map, const void* base, uint64_t blocks, uint64_t H
 // Makes `device` current for one call and puts the caller's device back.
 struct DeviceScope {
     int before = -1;
+    bool changed = false;
     cudaError_t err;
     explicit DeviceScope(int device) {
         err = cudaGetDevice(&before);
-        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+        if (err != cudaSuccess || before == device) return;
+        err = cudaSetDevice(device);
+        changed = err == cudaSuccess;
     }
     ~DeviceScope() {
-        if (before >= 0) cudaSetDevice(before);
+        if (changed) cudaSetDevice(before);
     }
 };
 
@@ -2059,6 +2062,7 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
     PrefixGeometry geo{NG, B, Hq, Hkv, D, (sh->flags & WEAVER_FLAG_CAUSAL) != 0, (sh->flags & WEAVER_FLAG_PARTIALS) != 0,
                        q_indptr, group_indptr, prefix_indptr, suffix_indptr};
+    WEAVER_CUDA_TRY(prepare_prefix(D), "prefix kernel attributes");
     PrefixTables t;
     plan_prefix(geo, static_cast<uint32_t>(eng->prop.multiProcessorCount), &t);
     if (t.items16.size() > 0x7FFFFFFFull || t.items_tc.size() > 0x7FFFFFFFull)

@@ -418,6 +418,9 @@ struct PrefixTables {
     uint32_t max_slots = 0;  // of a merged row
 };
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t);
+// Shared-memory sizes of the kernels for head dimension D, once per device.
+cudaError_t prepare_prefix(uint32_t D);
+cudaError_t prepare_prefix_tc(uint32_t D);
 // The kernels of one run, in this order, each but the first a programmatic
 // dependent launch (after = true) of the one before.
 cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s);

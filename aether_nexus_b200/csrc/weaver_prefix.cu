@@ -484,12 +484,13 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
 namespace {
 
 template <int D>
+constexpr size_t rows16_smem() {
+    return 1024 + PxLayout<D>::kBytes;
+}
+
+template <int D>
 cudaError_t rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s) {
-    const size_t smem = 1024 + PxLayout<D>::kBytes;
-    cudaError_t e = cudaFuncSetAttribute(prefix_rows16_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    prefix_rows16_kernel<D><<<n_items, kPxThreads, smem, s>>>(a);
+    prefix_rows16_kernel<D><<<n_items, kPxThreads, rows16_smem<D>(), s>>>(a);
     return cudaGetLastError();
 }
 
@@ -500,6 +501,14 @@ cudaError_t merge(const PrefixArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+cudaError_t prepare_prefix(uint32_t D) {
+    const cudaError_t e = D == 128 ? cudaFuncSetAttribute(prefix_rows16_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                          static_cast<int>(rows16_smem<128>()))
+                                   : cudaFuncSetAttribute(prefix_rows16_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                          static_cast<int>(rows16_smem<64>()));
+    return e == cudaSuccess ? prepare_prefix_tc(D) : e;
+}
 
 cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStream_t s) {
     return a.D == 128 ? rows16<128>(a, n_items, s) : rows16<64>(a, n_items, s);

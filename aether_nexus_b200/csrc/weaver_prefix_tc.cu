@@ -704,16 +704,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
 }
 
 template <int D>
+constexpr size_t tc_smem() {
+    return 1024 + TcLayout<D>::kBytes;
+}
+
+template <int D>
 cudaError_t launch_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas, bool after,
                       cudaStream_t s) {
-    const size_t smem = 1024 + TcLayout<D>::kBytes;
-    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    return launch_pdl(prefix_tc_kernel<D>, dim3(n_ctas), dim3(kTcThreads), smem, after, s, tm_k, tm_v, a);
+    return launch_pdl(prefix_tc_kernel<D>, dim3(n_ctas), dim3(kTcThreads), tc_smem<D>(), after, s, tm_k, tm_v, a);
 }
 
 }  // namespace
+
+cudaError_t prepare_prefix_tc(uint32_t D) {
+    return D == 128 ? cudaFuncSetAttribute(prefix_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(tc_smem<128>()))
+                    : cudaFuncSetAttribute(prefix_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(tc_smem<64>()));
+}
 
 cudaError_t launch_prefix_tc(const PrefixArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t n_ctas, bool after,
                              cudaStream_t s) {

@@ -21,12 +21,16 @@ same queries.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
 from . import _native as N
 from .types import BLOCK_SIZE
-from .weaver import WeaverEngine, _dptr, _stream_handle
+from .weaver import WeaverEngine, raw_stream
+
+_VIEWS = struct.Struct("=12Q").pack  # weaver_prefix_views
+assert struct.calcsize("=12Q") == ctypes.sizeof(N.PrefixViewsC)
 
 
 def _indptr(name, x) -> np.ndarray:
@@ -67,12 +71,11 @@ class PrefixPlan:
         self._h = h
         self.device, self.partials = engine.device, partials
         self.n_tokens, self.n_prefix_pages, self.n_suffix_pages = int(qi[-1]), int(pi[-1]), int(si[-1])
-
-    def _stream(self, stream):
-        if stream is None:  # the current stream of the object's device, which need not be the current one
-            import torch
-            stream = torch.cuda.current_stream(self.device)
-        return _stream_handle(stream)
+        import torch
+        self._f16, self._f32, self._words = (torch.float16,), (torch.float32,), (torch.int32, torch.uint32)
+        self.n_groups, self.n_seqs = gi.size - 1, B
+        self._heads, self._page = (q_heads, head_dim), (BLOCK_SIZE, kv_heads, head_dim)
+        self._rows, self._values = self.n_tokens * q_heads, self.n_tokens * q_heads * head_dim
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -89,57 +92,46 @@ class PrefixPlan:
     def kernel_count(self) -> int:
         return N.lib().weaver_prefix_plan_kernel_count(self._h)
 
-    def _check(self, name, t, dtypes, numel, shape=None):
+    def _ptr(self, name, t, dtypes, numel, tail=None):
         if t is None or isinstance(t, int):
-            return t
-        if not t.is_cuda or t.device.index != self.device:
+            return t or 0
+        if t.get_device() != self.device:
             raise ValueError(f"{name} must be a CUDA tensor on device {self.device}")
         if t.dtype not in dtypes:
             raise ValueError(f"{name} is {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        if shape is not None and tuple(t.shape[-len(shape):]) != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [..., {', '.join(map(str, shape))}]")
+        if tail is not None and t.shape[1:] != tail:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [..., {', '.join(map(str, tail))}]")
         if t.numel() < numel:
             raise ValueError(f"{name} has {t.numel()} elements, the plan needs {numel}")
-        return t
+        return t.data_ptr()
 
     def views(self, *, q, hot_k, hot_v, prefix_refs=None, suffix_refs=None, prefix_lens=None, suffix_lens=None, out=None,
-              part_m=None, part_l=None, part_o=None, hot_pool_blocks=None) -> N.PrefixViewsC:
-        """The C views struct of CUDA tensors (kept for repeated runs): ``q`` /
-        ``out [tokens, Hq, d]`` f16, ``hot_k`` / ``hot_v [blocks, 16, Hkv, d]``
-        f16 (or raw pointers with ``hot_pool_blocks``), refs and lengths int32
-        or uint32, partials fp32."""
-        import torch
-        s = self.shape
-        heads, n = (int(s.q_heads), int(s.head_dim)), self.n_tokens * int(s.q_heads)
-        words = (torch.int32, torch.uint32)
-        page = (BLOCK_SIZE, int(s.kv_heads), int(s.head_dim))
-        v = N.PrefixViewsC()
-        v.q = _dptr(self._check("q", q, (torch.float16,), n * heads[1], heads))
-        v.hot_k = _dptr(self._check("hot_k", hot_k, (torch.float16,), 0, page))
-        v.hot_v = _dptr(self._check("hot_v", hot_v, (torch.float16,), 0, page))
+              part_m=None, part_l=None, part_o=None, hot_pool_blocks=None) -> bytes:
+        """The C views (``weaver_prefix_views``) of CUDA tensors, kept for
+        repeated runs: ``q`` / ``out [tokens, Hq, d]`` f16, ``hot_k`` / ``hot_v
+        [blocks, 16, Hkv, d]`` f16 (or raw pointers with ``hot_pool_blocks``),
+        refs and lengths int32 or uint32, partials fp32."""
         if hot_pool_blocks is None:
             if isinstance(hot_k, int):
                 raise ValueError("raw pool pointers need hot_pool_blocks")
-            hot_pool_blocks = 0 if hot_k is None else int(hot_k.shape[0])
+            hot_pool_blocks = 0 if hot_k is None else hot_k.shape[0]
         for name, pool in (("hot_k", hot_k), ("hot_v", hot_v)):
-            if hasattr(pool, "shape") and int(pool.shape[0]) < hot_pool_blocks:
+            if hasattr(pool, "shape") and pool.shape[0] < hot_pool_blocks:
                 raise ValueError(f"{name} has fewer than {hot_pool_blocks} blocks")
-        v.hot_pool_blocks = hot_pool_blocks
-        v.prefix_refs = _dptr(self._check("prefix_refs", prefix_refs, words, self.n_prefix_pages))
-        v.suffix_refs = _dptr(self._check("suffix_refs", suffix_refs, words, self.n_suffix_pages))
-        v.prefix_lens = _dptr(self._check("prefix_lens", prefix_lens, words, int(s.num_groups)))
-        v.suffix_lens = _dptr(self._check("suffix_lens", suffix_lens, words, int(s.num_seqs)))
-        f32 = (torch.float32,)
-        v.out = _dptr(self._check("out", out, (torch.float16,), n * heads[1], heads))
-        v.part_m = _dptr(self._check("part_m", part_m, f32, n))
-        v.part_l = _dptr(self._check("part_l", part_l, f32, n))
-        v.part_o = _dptr(self._check("part_o", part_o, f32, n * heads[1]))
-        return v
+        ptr, n = self._ptr, self._rows
+        return _VIEWS(ptr("q", q, self._f16, self._values, self._heads), ptr("hot_k", hot_k, self._f16, 0, self._page),
+                      ptr("hot_v", hot_v, self._f16, 0, self._page), hot_pool_blocks,
+                      ptr("prefix_refs", prefix_refs, self._words, self.n_prefix_pages),
+                      ptr("suffix_refs", suffix_refs, self._words, self.n_suffix_pages),
+                      ptr("prefix_lens", prefix_lens, self._words, self.n_groups),
+                      ptr("suffix_lens", suffix_lens, self._words, self.n_seqs),
+                      ptr("out", out, self._f16, self._values, self._heads), ptr("part_m", part_m, self._f32, n),
+                      ptr("part_l", part_l, self._f32, n), ptr("part_o", part_o, self._f32, self._values))
 
-    def run_views(self, views: N.PrefixViewsC, stream=None) -> None:
-        N.check(N.lib().weaver_prefix_run(self._h, ctypes.byref(views), self._stream(stream)))
+    def run_views(self, views: bytes, stream=None) -> None:
+        N.check(N.lib().weaver_prefix_run(self._h, views, raw_stream(stream, self.device)))
 
     def run(self, stream=None, **tensors) -> None:
         """One attention over the batch on ``stream`` (default: torch's current

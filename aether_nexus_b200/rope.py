@@ -23,14 +23,18 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 
 from . import _native as N
 from .types import BLOCK_SIZE, REF_MASK
-from .weaver import _dptr, _stream_handle
+from .weaver import raw_stream
 
 LAYOUTS = {"half": N.ROPE_HALF, "interleaved": N.ROPE_INTERLEAVED}
+# weaver_rope_views as bytes in one go: a call made every layer spends its time in the host
+_VIEWS = struct.Struct("=4I3Q6Q3QfI2Q4Q4QQ").pack
+assert struct.calcsize("=4I3Q6Q3QfI2Q4Q4QQ") == ctypes.sizeof(N.RopeViewsC)
 
 
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[np.ndarray, float]:
@@ -119,6 +123,7 @@ class Rope:
 
     def __init__(self, engine, *, head_dim: int, rot_dim: int | None = None, theta: float = 10000.0,
                  layout: str = "half", scaling: dict | None = None, inv_freq=None, amplitude: float | None = None):
+        import torch
         rot_dim = head_dim if rot_dim is None else int(rot_dim)
         if layout not in LAYOUTS:
             raise ValueError(f"layout {layout!r}, not one of {sorted(LAYOUTS)}")
@@ -137,12 +142,8 @@ class Rope:
         h = ctypes.c_void_p()
         N.check(N.lib().weaver_rope_create(engine.handle, ctypes.byref(c), ctypes.byref(h)))
         self._h = h
-
-    def _stream(self, stream):
-        if stream is None:  # the current stream of the object's device, which need not be the current one
-            import torch
-            stream = torch.cuda.current_stream(self.device)
-        return _stream_handle(stream)
+        self._types = {torch.float16: N.F16, torch.bfloat16: N.BF16}
+        self._f16, self._i32, self._i64 = torch.float16, torch.int32, torch.int64
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -155,41 +156,52 @@ class Rope:
         except Exception:
             pass
 
-    def _check(self, name, t, shape, dtype):
-        if not t.is_cuda or t.device.index != self.device:
+    def _refuse(self, name, t, shape, dtype):
+        """Says what is wrong with a tensor that failed its check."""
+        if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{name} must be a CUDA tensor on device {self.device}")
-        if dtype is not None and t.dtype != dtype:
+        if t.dtype != dtype:
             raise ValueError(f"{name} is {t.dtype}, not {dtype}")
         if tuple(t.shape) != tuple(shape):
             raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"the last dimension of {name} must be contiguous")
-        return t
+        raise ValueError(f"the last dimension of {name} must be contiguous")
 
-    def _views(self, q, k, positions, q_weight, k_weight, eps) -> N.RopeViewsC:
-        import torch
-        if q is None and k is None:
-            raise ValueError("neither q nor k given")
+    def _heads(self, name, t, shape, dtype):
+        """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+        st = t.stride() if t.dim() == 3 else (0, 0, 0)
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self.device or st[2] != 1:
+            self._refuse(name, t, shape, dtype)
+        return t.data_ptr(), st[0], st[1]
+
+    def _flat(self, name, t, n, dtype):
+        if t.shape != (n,) or t.dtype != dtype or t.get_device() != self.device or (n > 1 and t.stride(0) != 1):
+            self._refuse(name, t, (n,), dtype)
+        return t.data_ptr()
+
+    def _inputs(self, q, k, positions, q_weight, k_weight, q_out, out_dtype):
+        """Tokens, heads, type code, and the views of q, k, positions, the weights and q_out."""
         lead = q if q is not None else k
+        if lead is None:
+            raise ValueError("neither q nor k given")
         if lead.dim() != 3:
             raise ValueError("heads are [tokens, heads, head_dim] tensors")
-        T, dt = int(lead.shape[0]), lead.dtype
-        if dt not in (torch.float16, torch.bfloat16):
+        dt, T, d = lead.dtype, lead.shape[0], self.head_dim
+        if dt not in self._types:
             raise ValueError(f"heads are {dt}, not float16 or bfloat16")
-        v = N.RopeViewsC()
-        v.n_tokens, v.dtype, v.eps = T, N.F16 if dt == torch.float16 else N.BF16, float(eps)
+        hq, qv, qo = 0, (0, 0, 0), (0, 0, 0)
         if q is not None:
-            self._check("q", q, (T, q.shape[1], self.head_dim), dt)
-            v.q, v.q_heads, v.q_token_stride, v.q_head_stride = q.data_ptr(), q.shape[1], q.stride(0), q.stride(1)
+            hq = q.shape[1]
+            qv = self._heads("q", q, (T, hq, d), dt)
+            qo = self._heads("q_out", q_out, (T, hq, d), out_dtype or dt)
+        hkv, kv = 0, (0, 0, 0)
         if k is not None:
-            self._check("k", k, (T, k.shape[1], self.head_dim), dt)
-            v.k, v.kv_heads, v.k_token_stride, v.k_head_stride = k.data_ptr(), k.shape[1], k.stride(0), k.stride(1)
-        self._check("positions", positions, (T,), torch.int32)
-        v.positions = positions.data_ptr()
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None:
-                setattr(v, name, self._check(name, w, (self.head_dim,), dt).data_ptr())
-        return v
+            if k.dim() != 3:
+                raise ValueError("heads are [tokens, heads, head_dim] tensors")
+            hkv = k.shape[1]
+            kv = self._heads("k", k, (T, hkv, d), dt)
+        return (T, hq, hkv, dt, qv, kv, qo, self._flat("positions", positions, T, self._i32),
+                0 if q_weight is None else self._flat("q_weight", q_weight, d, dt),
+                0 if k_weight is None else self._flat("k_weight", k_weight, d, dt))
 
     def rotate(self, q, k, positions, q_out, k_out=None, *, q_weight=None, k_weight=None, eps: float = 1e-6,
                stream=None) -> None:
@@ -197,14 +209,11 @@ class Rope:
         rotated) ``q [T, Hq, d]`` / ``k [T, Hkv, d]`` (float16 or bfloat16, any
         token and head strides; outputs of the inputs' type, the input itself
         included).  ``q`` or ``k`` may be None.  ``positions [T]`` int32."""
-        v = self._views(q, k, positions, q_weight, k_weight, eps)
-        if q is not None:
-            self._check("q_out", q_out, q.shape, q.dtype)
-            v.q_out, v.q_out_token_stride, v.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-        if k is not None:
-            self._check("k_out", k_out, k.shape, k.dtype)
-            v.k_out, v.k_out_token_stride, v.k_out_head_stride = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
-        N.check(N.lib().weaver_rope_rotate(self._h, ctypes.byref(v), self._stream(stream)))
+        T, hq, hkv, dt, qv, kv, qo, pos, qw, kw = self._inputs(q, k, positions, q_weight, k_weight, q_out, None)
+        ko = (0, 0, 0) if k is None else self._heads("k_out", k_out, (T, hkv, self.head_dim), dt)
+        raw = _VIEWS(T, hq, hkv, self._types[dt], qv[0], kv[0], 0, qv[1], qv[2], kv[1], kv[2], 0, 0, pos, qw, kw, eps, 0,
+                     qo[0], ko[0], qo[1], qo[2], ko[1], ko[2], 0, 0, 0, 0, 0)
+        N.check(N.lib().weaver_rope_rotate(self._h, raw, raw_stream(stream, self.device)))
 
     def append(self, q, k, v, positions, slots, hot_k, hot_v, q_out, bad_flag, *, q_weight=None, k_weight=None,
                eps: float = 1e-6, hot_pool_blocks: int | None = None, stream=None) -> None:
@@ -216,37 +225,36 @@ class Rope:
         ``DeviceFabric`` layer's) with ``hot_pool_blocks``.  ``bad_flag`` (one
         int32) gets 1 OR-ed in for a slot beyond the pool, whose token is
         skipped.  The slots of one call must be distinct."""
-        import torch
         if k is None:
             raise ValueError("append needs k")
-        x = self._views(q, k, positions, q_weight, k_weight, eps)
-        T, hkv = int(k.shape[0]), int(k.shape[1])
-        if q is not None:
-            self._check("q_out", q_out, q.shape, torch.float16)
-            x.q_out, x.q_out_token_stride, x.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+        T, hq, hkv, dt, qv, kv, qo, pos, qw, kw = self._inputs(q, k, positions, q_weight, k_weight, q_out, self._f16)
         if (v is None) != (hot_v is None):
             raise ValueError("v and hot_v come together")
-        if v is not None:
-            self._check("v", v, k.shape, k.dtype)
-            x.v, x.v_token_stride, x.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
-        blocks = hot_pool_blocks
-        for name, pool in (("hot_k", hot_k), ("hot_v", hot_v)):
+        vv = (0, 0, 0) if v is None else self._heads("v", v, (T, hkv, self.head_dim), dt)
+        blocks, pools = hot_pool_blocks, [0, 0]
+        for i, pool in enumerate((hot_k, hot_v)):
             if pool is None or isinstance(pool, int):
+                pools[i] = pool or 0
                 continue
-            self._check(name, pool, (pool.shape[0], BLOCK_SIZE, hkv, self.head_dim), torch.float16)
+            name, n = ("hot_k", "hot_v")[i], pool.shape[0]
+            if pool.shape != (n, BLOCK_SIZE, hkv, self.head_dim) or pool.dtype != self._f16 or \
+                    pool.get_device() != self.device:
+                self._refuse(name, pool, (n, BLOCK_SIZE, hkv, self.head_dim), self._f16)
             if not pool.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
             if blocks is None:
-                blocks = int(pool.shape[0])
-            if int(pool.shape[0]) < blocks:
+                blocks = n
+            if n < blocks:
                 raise ValueError(f"{name} has fewer than {blocks} blocks")
+            pools[i] = pool.data_ptr()
         if blocks is None:
             raise ValueError("raw pool pointers need hot_pool_blocks")
-        self._check("slots", slots, (T,), torch.int64)
-        self._check("bad_flag", bad_flag.reshape(-1)[:1], (1,), torch.int32)
-        x.slots, x.bad_flag = slots.data_ptr(), bad_flag.data_ptr()
-        x.hot_k, x.hot_v, x.hot_pool_blocks = _dptr(hot_k), _dptr(hot_v), blocks
-        N.check(N.lib().weaver_rope_append(self._h, ctypes.byref(x), self._stream(stream)))
+        if bad_flag.dtype != self._i32 or bad_flag.numel() < 1 or bad_flag.get_device() != self.device:
+            raise ValueError(f"bad_flag must be an int32 CUDA tensor on device {self.device}")
+        raw = _VIEWS(T, hq, hkv, self._types[dt], qv[0], kv[0], vv[0], qv[1], qv[2], kv[1], kv[2], vv[1], vv[2], pos, qw, kw,
+                     eps, 0, qo[0], 0, qo[1], qo[2], 0, 0, self._flat("slots", slots, T, self._i64), pools[0], pools[1],
+                     blocks, bad_flag.data_ptr())
+        N.check(N.lib().weaver_rope_append(self._h, raw, raw_stream(stream, self.device)))
 
 
 __all__ = ["Rope", "rope_frequencies", "token_slots"]

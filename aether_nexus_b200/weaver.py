@@ -136,6 +136,16 @@ def _stream_handle(stream):
     return stream.cuda_stream
 
 
+def raw_stream(stream, device: int) -> int:
+    """The ``cudaStream_t`` of ``stream``, or of the current stream of
+    ``device`` (which need not be the current device)."""
+    if stream is None:
+        import torch
+        fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a tenth of the Stream object's time
+        return fast(device) if fast else torch.cuda.current_stream(device).cuda_stream
+    return _stream_handle(stream)
+
+
 class WeaverPlan:
     """A decode-step plan over device-resident pools (``weaver_plan_create``).
 
