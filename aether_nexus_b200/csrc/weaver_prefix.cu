@@ -14,8 +14,8 @@
 // A plan cuts every (list, kv head, row tile) into items along the pages, so
 // that there are enough CTAs however few rows there are; each item writes its
 // rows' (m, l, o) and the merge joins them.  A tile with one item whose rows
-// get nothing from elsewhere is written directly.  Lists of more than 16 rows
-// per kv head run on tcgen05 (weaver_prefix_tc.cu), the others here:
+// get nothing from elsewhere is written directly.  Lists of more than 8 or 16
+// rows per kv head run on tcgen05 (weaver_prefix_tc.cu), the others here:
 //
 // prefix_rows16_kernel: tiles of 16 rows on mma.sync, as the multi-query
 // attention of the flat caches: four warps take every fourth 16-token page of
@@ -279,9 +279,13 @@ __global__ void __launch_bounds__(8 * D / 4) prefix_merge_kernel(const __grid_co
 constexpr uint32_t kOwnRows = 512;
 // Starting an item (query rows in, results out, the pipeline filling) in the
 // units of a token tile's cost.
-constexpr uint32_t kItemCost = 24;
-// Up to 16 rows a 16-row tile costs one pass over the pages either way.
-constexpr uint32_t kRows16 = 16;
+constexpr uint32_t kItemCost = 48;
+// Lists of up to 16 rows go to the 16-row tiles, whose many small CTAs start
+// and end faster than items of the tensor-memory kernel; lists of 9 to 16 rows
+// only where they are many (more than two tiles an SM), since a few more items
+// there cost less than another kernel (8 sequences x 4 queries of 4 heads: 23
+// us on tensor memory, 31 with both; 200 sequences x 3: 129 and 94).
+constexpr uint32_t kRows16 = 16, kRowsFew = 8;
 
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     const uint32_t G = geo.Hq / geo.Hkv, NG = geo.n_groups, B = geo.n_seqs, none = ~0u;
@@ -340,12 +344,16 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         if (x.x != none && pages(x.x) && x.z != none && pages(x.z)) joined[x.x] = joined[x.z] = 1;
 
     // tiles, and the work of either kind
+    uint64_t mid = 0;
+    for (uint32_t l = 0; l < n_lists; ++l)
+        if (pages(l) && rows_of(l) > kRowsFew && rows_of(l) <= kRows16) mid += geo.Hkv;
+    const uint64_t most_rows16 = mid > 2ull * n_sm ? kRows16 : kRowsFew;
     struct TcTile { uint32_t tile, n, cost; };
     std::vector<TcTile> tc;
     uint64_t work16 = 0, cost_tc = 0, n_tc = 0;
     for (uint32_t l = 0; l < n_lists; ++l) {
         PrefixList& L = t->lists[l];
-        const bool small = rows_of(l) <= kRows16;
+        const bool small = rows_of(l) <= most_rows16;
         L.tile_rows = small ? 16 : 256;
         L.n_tiles = static_cast<uint32_t>((rows_of(l) + L.tile_rows - 1) / L.tile_rows);
         L.tile0 = static_cast<uint32_t>(t->tiles.size());
@@ -393,9 +401,11 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         return it;
     };
 
-    // 16-row tiles: about three CTAs fit an SM; items of whole multiples of
-    // four pages (one per warp), as long as that still gives two full waves
-    const uint64_t target = 6ull * n_sm;
+    // 16-row tiles: three CTAs fit an SM; items of whole multiples of four pages
+    // (one per warp), one full wave of them where there are pages enough (74 MB
+    // of own pages of 40 sequences: 82.6 us a run with two waves, 81.4 with one,
+    // 92.7 with four: an item's start and end cost as much as several pages)
+    const uint64_t target = 3ull * n_sm;
     const uint64_t per = std::max<uint64_t>(4, ((work16 + target - 1) / target + 3) / 4 * 4);
     for (uint32_t ti = 0; ti < t->tiles.size(); ++ti) {
         PrefixTile& T = t->tiles[ti];
