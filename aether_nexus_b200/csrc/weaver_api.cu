@@ -1880,6 +1880,12 @@ struct DeviceScope {
     }
 };
 
+// Two regions of `bytes` bytes with some in common.
+bool overlap(const void* x, const void* y, uint64_t bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return (a > b ? a - b : b - a) < bytes;
+}
+
 // An output [T][H][D] whose elements do not overlap.
 bool disjoint_rows(uint64_t T, uint64_t H, uint64_t D, uint64_t ts, uint64_t hs) {
     if (T == 0 || H == 0) return true;
@@ -1892,12 +1898,12 @@ bool disjoint_rows(uint64_t T, uint64_t H, uint64_t D, uint64_t ts, uint64_t hs)
 int rope_output(const char* name, const void* in, uint64_t in_ts, uint64_t in_hs, const void* out, uint64_t ts,
                 uint64_t hs, uint64_t T, uint64_t H, uint64_t D) {
     if (!in || !out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s or its output is null", name);
-    if (!aligned16(in) || !aligned16(out) || in_ts % 8 || in_hs % 8 || ts % 8 || hs % 8)
+    if (!aligned16(in) || !aligned16(out) || (T > 1 && (in_ts % 8 || ts % 8)) || (H > 1 && (in_hs % 8 || hs % 8)))
         return fail(WEAVER_ERR_MISALIGNED, "%s rows not 16-byte aligned", name);
     if (!disjoint_rows(T, H, D, ts, hs)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "rows of %s's output overlap", name);
     const char* i0 = static_cast<const char*>(in);
     const char* o0 = static_cast<const char*>(out);
-    if (T && H && !(in == out && in_ts == ts && in_hs == hs)) {  // the same rows, or none in common
+    if (T && H && !(in == out && (T == 1 || in_ts == ts) && (H == 1 || in_hs == hs))) {  // the same rows, or none in common
         const char* i1 = i0 + 2 * ((T - 1) * in_ts + (H - 1) * in_hs + D);
         const char* o1 = o0 + 2 * ((T - 1) * ts + (H - 1) * hs + D);
         if (i0 < o1 && o0 < i1)
@@ -1929,12 +1935,13 @@ int rope_run(weaver_rope* rope, const weaver_rope_views* v, void* stream, bool a
         if (!v->kv_heads || !v->k || !v->hot_k || !v->slots || !v->bad_flag)
             return fail(WEAVER_ERR_INVALID_ARGUMENT, "append needs k, hot_k, slots and bad_flag");
         if (!v->v != !v->hot_v) return fail(WEAVER_ERR_INVALID_ARGUMENT, "v and hot_v come together");
-        if (v->hot_k == v->hot_v)
-            return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_v is hot_k: pass v and hot_v null for a pool shared by K and V");
         if (v->hot_pool_blocks == 0 || v->hot_pool_blocks > (1ull << 31))
             return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_pool_blocks %llu", (unsigned long long)v->hot_pool_blocks);
+        if (v->hot_v && overlap(v->hot_k, v->hot_v, v->hot_pool_blocks * kBlock * v->kv_heads * D * 2))
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "hot_v overlaps hot_k: pass v and hot_v null for a pool shared by K and V");
         if (!aligned16(v->k) || !aligned16(v->v) || !aligned16(v->hot_k) || !aligned16(v->hot_v) ||
-            v->k_token_stride % 8 || v->k_head_stride % 8 || (v->v && (v->v_token_stride % 8 || v->v_head_stride % 8)))
+            (T > 1 && (v->k_token_stride % 8 || (v->v && v->v_token_stride % 8))) ||
+            (v->kv_heads > 1 && (v->k_head_stride % 8 || (v->v && v->v_head_stride % 8))))
             return fail(WEAVER_ERR_MISALIGNED, "k, v or the pool not 16-byte aligned");
         if ((reinterpret_cast<uintptr_t>(v->slots) & 7u) || (reinterpret_cast<uintptr_t>(v->bad_flag) & 3u))
             return fail(WEAVER_ERR_MISALIGNED, "slots or bad_flag misaligned");
@@ -2148,6 +2155,8 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
     } else {
         if (!v->out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "views.out is null");
         if (!aligned16(v->out)) return fail(WEAVER_ERR_MISALIGNED, "out not 16-byte aligned");
+        if (v->q && overlap(v->q, v->out, static_cast<uint64_t>(a.n_tokens) * a.Hq * a.D * 2))
+            return fail(WEAVER_ERR_INVALID_ARGUMENT, "out overlaps q");
         a.out = static_cast<__half*>(v->out);
     }
     if (plan->n_prefix_pages + plan->n_suffix_pages) {

@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         const uint32_t lanes = (warp & 3) * 32;  // this warp's rows: tensor-memory lanes
         const uint32_t ts = tmem + (lanes << 16) + h * 128, to = tmem + (lanes << 16) + L::kO + h * D;
         uint8_t* const qh = qs + h * L::kQ;
-        const float scale2 = fabsf(a.scale) * kLog2e;
+        // a scale of 0 is a query of zeros (0 times the -inf of a masked score is NaN)
+        const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
         constexpr uint32_t kChunks = D / 8, kStep = 32 / kChunks;  // 16-byte chunks of a row; rows per warp-wide copy
         const uint32_t ch = lane % kChunks, sub = lane / kChunks;
         uint32_t k = 0;  // tiles so far
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 for (uint32_t y = sub; y < 32; y += kStep) {
                     const uint64_t row = __shfl_sync(0xffffffffu, at, y);
                     cp_async16_zfill(qh + (ch >> 3) * 16384 + swz128(lanes + y, ch & 7), a.q + row * D + ch * 8,
-                                     lanes + y < mine);
+                                     lanes + y < mine && a.scale != 0.0f);
                 }
                 cp_async_wait_all();
                 if (a.scale < 0.0f) {  // a negative scale goes into Q: each lane flips what it copied

@@ -480,14 +480,14 @@ typedef struct weaver_rope_config {
     const double* inv_freq; /* host, rot_dim / 2 values: radians per position */
 } weaver_rope_config;
 
-/* Strides are in elements, multiples of 8; a head's head_dim elements are
- * contiguous.  All pointers 16-byte aligned device pointers. */
+/* Strides are in elements, multiples of 8 (0 included for inputs, any value
+ * where there is one token or head); a head's head_dim elements are contiguous.  All pointers 16-byte aligned device pointers. */
 typedef struct weaver_rope_views {
     uint32_t n_tokens, q_heads, kv_heads;
     uint32_t dtype;            /* weaver_dtype of q, k, v and the weights */
     const void* q;             /* [n_tokens][q_heads][head_dim]; null with q_heads = 0 */
     const void* k;             /* [n_tokens][kv_heads][head_dim]; null with kv_heads = 0 */
-    const void* v;             /* append only; null with hot_v (the pool's one region for K and V) */
+    const void* v;             /* append only; null with hot_v (a pool whose one region serves K and V) */
     uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
     const int32_t* positions;  /* [n_tokens], negative ones included */
     const void* q_weight;      /* [head_dim], or null: no norm of the query heads */
@@ -532,8 +532,10 @@ WEAVER_EXPORT int weaver_rope_append(weaver_rope* rope, const weaver_rope_views*
  * One token per sequence, draft batches and prompt chunks may be mixed; a
  * group of one sequence with no prefix is a plain paged sequence.
  *
- * The tokens of the last page past a length, and pages past it, are not part
- * of the result whatever the pool holds there.  A NaN or infinite value at a
+ * Rows of q and out behind the last query are not touched; out and q do not
+ * overlap; the lengths and references stay as they are while a run is in
+ * flight.  The tokens of the last page past a length, and pages past it, are not
+ * part of the result whatever the pool holds there.  A NaN or infinite value at a
  * position that some query of a call sees can turn the outputs of other
  * queries of that head NaN too, causally masked or not.
  * WEAVER_FLAG_PARTIALS writes (m, l, o) instead of out, as weaver_run does, so

@@ -358,3 +358,45 @@ def test_null_views_are_refused(engine):
         with pytest.raises(W.WeaverError) as e:
             plan.run(**b.views(**{name: getattr(b, name).data_ptr() + 2}))
         assert e.value.status == 3
+
+
+def test_out_over_q_is_refused(engine):
+    b = Batch([(32, [(2, 16)])], 4, 1, 64, seed=16)
+    plan = b.plan(engine)
+    with pytest.raises(W.WeaverError) as e:
+        plan.run(**b.views(out=b.q))
+    assert e.value.status == 1
+
+
+@pytest.mark.parametrize("shape", ["drafts", "prompts", "many_sequences"])
+def test_rows_behind_the_last_query_are_left_alone(engine, shape):
+    """A batch padded behind its last query: the padding of out keeps what it held."""
+    import torch
+    b = Batch(SHAPES[shape], 8, 2, 128, seed=17)
+    pad = torch.full((9,) + tuple(b.q.shape[1:]), math.nan, dtype=torch.float16, device="cuda")
+    out = torch.full((b.T + 9,) + tuple(b.q.shape[1:]), 3.0, dtype=torch.float16, device="cuda")
+    plan = b.plan(engine)
+    plan.run(**b.views(q=torch.cat([b.q, pad]), out=out))
+    plan.status()
+    b.check(out[:b.T])
+    assert (out[b.T:] == 3.0).all()
+
+
+def test_negative_and_zero_scale(engine):
+    """scale < 0 turns the order of the scores round, 0 weighs every token alike."""
+    b = Batch(SHAPES["prompts"], 8, 2, 64, seed=18)
+    q = b.q.clone()
+    for scale, factor in ((-b.d ** -0.5, -1.0), (0.0, 0.0)):
+        plan = b.plan(engine, scale=scale)
+        b.q = q
+        plan.run(**b.views())
+        plan.status()
+        b.q = q * factor  # the formula with scale d^-1/2 and the queries turned round
+        b.check()
+    b.q = q
+    small = Batch([(40, [(1, 9)])], 4, 1, 128, seed=19)  # the 16-row tiles too
+    plan = small.plan(engine, scale=-small.d ** -0.5)
+    plan.run(**small.views())
+    plan.status()
+    small.q = -small.q
+    small.check()

@@ -256,3 +256,37 @@ def test_python_refusals(engine, change):
     qo = torch.zeros(4, 8, 64, dtype=torch.float16, device="cuda")
     with pytest.raises(ValueError):
         rope.append(a["q"], a["k"], a["v"], a["positions"], a["slots"], a["pool"][0], a["pool"][1], qo, bad)
+
+
+def test_one_token_of_any_stride(engine):
+    """With one token its stride does not matter (a slice whose stride is odd)."""
+    import torch
+    wide = torch.zeros(2, 8 * 64 + 3, dtype=torch.float16, device="cuda")
+    q = wide[:1, :512].view(1, 8, 64)
+    q.copy_(heads(1, 8, 64, torch.float16, 1))
+    out = torch.empty(1, 8, 64, dtype=torch.float16, device="cuda")
+    pos = torch.tensor([5], dtype=torch.int32, device="cuda")
+    rope = W.Rope(engine, head_dim=64)
+    rope.rotate(q, None, pos, out)
+    check(out, *reference(q, pos, rope.inv_freq, 1.0, 64, "half"))
+
+
+def test_broadcast_heads_as_input(engine):
+    """One key head given to four by a stride of zero."""
+    import torch
+    k = heads(6, 1, 128, torch.bfloat16, 2).expand(6, 4, 128)
+    out = torch.empty(6, 4, 128, dtype=torch.bfloat16, device="cuda")
+    pos = torch.arange(6, device="cuda", dtype=torch.int32)
+    rope = W.Rope(engine, head_dim=128)
+    rope.rotate(None, k, pos, None, out)
+    check(out, *reference(k, pos, rope.inv_freq, 1.0, 128, "half"))
+
+
+def test_no_tokens(engine):
+    import torch
+    e = torch.empty(0, 4, 64, dtype=torch.float16, device="cuda")
+    pool = torch.zeros(1, 16, 4, 64, dtype=torch.float16, device="cuda")
+    rope = W.Rope(engine, head_dim=64)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    rope.rotate(e, e, none, e, e)
+    rope.append(e, e, None, none, none.long(), pool, None, e, torch.zeros(1, dtype=torch.int32, device="cuda"))

@@ -127,7 +127,7 @@ def test_rotate_refuses(engine_memory, kw, status):
     (dict(k=None), INVALID), (dict(kv_heads=0), INVALID), (dict(slots=None), INVALID), (dict(bad_flag=None), INVALID),
     (dict(hot_k=None), INVALID), (dict(hot_v=None), INVALID), (dict(v=None), INVALID), (dict(hot_v=8 << 20), INVALID),
     (dict(hot_pool_blocks=0), INVALID), (dict(hot_k=(8 << 20) + 8), MISALIGNED), (dict(v_token_stride=252), MISALIGNED),
-    (dict(slots=(7 << 20) + 4), MISALIGNED)])
+    (dict(slots=(7 << 20) + 4), MISALIGNED), (dict(hot_v=(8 << 20) + 4096), INVALID)])
 def test_append_refuses(engine_memory, kw, status):
     rc, h = _rope(engine_memory)
     assert rc == 0
