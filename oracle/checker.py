@@ -138,7 +138,7 @@ def literal_decode(q_exact, q_latent, hot_pool, cold_pool, loom_refs, dictionary
             _ptr(dictionary), ctypes.byref(p), _ptr(out))
     else:
         hot_blocks = hot_pool.size // (16 * p.kv_heads * p.head_dim)
-        cold_blocks = cold_pool.size // (16 * p.kv_heads)
+        cold_blocks = cold_pool.size // (16 * p.kv_heads * SPARSE_CODE_DTYPE.itemsize)
         rc = lib().oracle_literal_decode(
             _ptr(q_exact), _ptr(q_latent), _ptr(hot_pool), ctypes.c_uint64(hot_blocks),
             _ptr(cold_pool), ctypes.c_uint64(cold_blocks), _ptr(loom_refs), _ptr(dictionary),

@@ -74,6 +74,20 @@ def test_literal_out_of_range_ref_is_refused(oracle_mod):
         oracle_mod.literal_decode(*[w[k] for k in LITERAL_KEYS], w["params"])
 
 
+def test_literal_pool_bound_counts_codes_not_bytes(oracle_mod):
+    """The records behind the pool's end are zeros here, which decode without
+    an error: only the bound itself can refuse the reference."""
+    w = make_golden.literal_inputs(make_golden.LITERAL_CASES["lit_g4_seed0"])
+    pool = np.ascontiguousarray(w["cold_pool"]).reshape(-1)
+    longer = np.zeros(8 * pool.size, dtype=pool.dtype)
+    longer[:pool.size] = pool
+    w["cold_pool"] = longer[:pool.size]
+    w["loom_refs"] = w["loom_refs"].copy()
+    w["loom_refs"][-1] = 2  # the first block behind a pool of 2
+    with pytest.raises(ValueError):
+        oracle_mod.literal_decode(*[w[k] for k in LITERAL_KEYS], w["params"])
+
+
 def _config_case(name):
     c = dict(make_golden.CONFIG_CASES[name])
     return synth.make_workload(c.pop("cfg"), c.pop("seed"), flag_refs=c.pop("flag_refs", False), **c)
