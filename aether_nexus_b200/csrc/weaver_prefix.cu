@@ -26,6 +26,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <functional>
+#include <queue>
 #include <stdexcept>
 
 #include "weaver_device.cuh"
@@ -287,6 +289,39 @@ constexpr uint32_t kItemCost = 48;
 // us on tensor memory, 31 with both; 200 sequences x 3: 129 and 94).
 constexpr uint32_t kRows16 = 16, kRowsFew = 8;
 
+// The length of a 16-row item, in pages: that of least makespan on `slots`
+// resident CTAs, where an item costs kStart16 rounds beside a round for every
+// four of its pages (a page per warp).  64 sequences behind one prefix, 38 MB of
+// own pages: 67.4 us a run where the item only divided the work by the slots,
+// 65.6 so (69.9 with a start of one round, the same with 3 to 12); 40 sequences,
+// 123 MB: 81.0 and 77.2.
+constexpr uint64_t kStart16 = 6;
+static uint64_t rows16_item(const std::vector<uint64_t>& tiles, uint64_t slots) {
+    uint64_t longest = 1, total = 0;
+    for (uint64_t n : tiles) longest = std::max(longest, n), total += n;
+    uint64_t best = 4, least = ~0ull;
+    // no shorter than four waves of equal items, then in steps of an eighth
+    for (uint64_t per = std::max<uint64_t>(4, total / (4 * slots) / 4 * 4);; per += std::max<uint64_t>(4, per / 8 / 4 * 4)) {
+        std::vector<uint64_t> cost;
+        for (uint64_t n : tiles) {
+            const uint64_t k = (n + per - 1) / per;
+            for (uint64_t s = 0; s < k; ++s) cost.push_back(kStart16 + (n * (s + 1) / k - n * s / k + 3) / 4);
+        }
+        std::sort(cost.begin(), cost.end(), std::greater<uint64_t>());
+        std::priority_queue<uint64_t, std::vector<uint64_t>, std::greater<uint64_t>> ends;
+        uint64_t span = 0;
+        for (uint64_t c : cost) {
+            uint64_t from = 0;
+            if (ends.size() == slots) from = ends.top(), ends.pop();
+            ends.push(from + c);
+            span = std::max(span, from + c);
+        }
+        if (span < least) least = span, best = per;
+        if (per >= longest) break;
+    }
+    return best;
+}
+
 void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     const uint32_t G = geo.Hq / geo.Hkv, NG = geo.n_groups, B = geo.n_seqs, none = ~0u;
     // (list, token of it) of every token's pooled part and of its own part
@@ -350,7 +385,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     const uint64_t most_rows16 = mid > 2ull * n_sm ? kRows16 : kRowsFew;
     struct TcTile { uint32_t tile, n, cost; };
     std::vector<TcTile> tc;
-    uint64_t work16 = 0, cost_tc = 0, n_tc = 0;
+    uint64_t cost_tc = 0, n_tc = 0;
     for (uint32_t l = 0; l < n_lists; ++l) {
         PrefixList& L = t->lists[l];
         const bool small = rows_of(l) <= most_rows16;
@@ -366,9 +401,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
                 T.kvh = g;
                 T.row0 = r * L.tile_rows;
                 T.rows = static_cast<uint32_t>(std::min<uint64_t>(L.tile_rows, rows_of(l) - T.row0));
-                if (small) {
-                    work16 += pages(l);
-                } else {
+                if (!small) {
                     // token tiles below the causal limit of the tile's last
                     // row, the pages taken as full
                     uint64_t own = static_cast<uint64_t>(L.suf_blocks) * kBlock;
@@ -401,12 +434,13 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         return it;
     };
 
-    // 16-row tiles: three CTAs fit an SM; items of whole multiples of four pages
-    // (one per warp), one full wave of them where there are pages enough (74 MB
-    // of own pages of 40 sequences: 82.6 us a run with two waves, 81.4 with one,
-    // 92.7 with four: an item's start and end cost as much as several pages)
-    const uint64_t target = 3ull * n_sm;
-    const uint64_t per = std::max<uint64_t>(4, ((work16 + target - 1) / target + 3) / 4 * 4);
+    // 16-row tiles: items of whole multiples of four pages (one per warp), three
+    // CTAs to an SM at a time.  Of the possible item lengths the one whose items
+    // end first when dealt out longest first, as the grid is.
+    std::vector<uint64_t> sizes;
+    for (const PrefixTile& T : t->tiles)
+        if (t->lists[T.list].tile_rows == 16) sizes.push_back(pages(T.list));
+    const uint64_t per = rows16_item(sizes, 3 * n_sm);
     for (uint32_t ti = 0; ti < t->tiles.size(); ++ti) {
         PrefixTile& T = t->tiles[ti];
         if (t->lists[T.list].tile_rows != 16) continue;
@@ -417,13 +451,15 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         for (uint32_t s = 0; s < T.n_slots; ++s) {
             PrefixItem it = item_of(T, 1);
             it.part_row = part_rows + s * rows;
-            it.t0 = static_cast<uint32_t>(s * per);
-            it.t1 = static_cast<uint32_t>(std::min<uint64_t>(n, (s + 1) * per));
+            it.t0 = static_cast<uint32_t>(n * s / T.n_slots);
+            it.t1 = static_cast<uint32_t>(n * (s + 1) / T.n_slots);
             it.flags |= T.direct ? kPxDirect : 0;
             t->items16.push_back(it);
         }
         if (!T.direct) part_rows += T.n_slots * rows;
     }
+    std::stable_sort(t->items16.begin(), t->items16.end(),
+                     [](const PrefixItem& x, const PrefixItem& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
 
     // tensor-memory tiles: one CTA per SM, each with an equal share of the
     // cost along the list of tiles, so a tile is cut only where a share ends
