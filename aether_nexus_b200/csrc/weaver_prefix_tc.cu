@@ -256,18 +256,30 @@ struct Work {
     static __device__ __forceinline__ uint32_t fetch(const PrefixArgs& a, uint32_t i, uint32_t end, uint32_t lane) {
         return i < end && lane < sizeof(PrefixItem) / 4 ? reinterpret_cast<const uint32_t*>(a.tc_items + i)[lane] : 0u;
     }
-    __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t word, bool report) {
+    // Tokens of the prefix and own pages that a record names: a load each, apart
+    // from the rest so that a role may have the next item's on their way.
+    struct Lens {
+        uint32_t pre, suf;
+    };
+    static __device__ __forceinline__ Lens lens(const PrefixArgs& a, uint32_t word, bool report) {
+        auto at = [&](uint32_t w) { return __shfl_sync(0xffffffffu, word, w); };
+        const uint32_t pre_blocks = at(8), pre_i = at(9), suf_blocks = at(12), suf_i = at(13);
+        return Lens{page_len(a.prefix_lens, pre_i, pre_blocks, a.status, report),
+                    page_len(a.suffix_lens, suf_i, suf_blocks, a.status, report)};
+    }
+    __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t word, bool report) : Work(a, word, lens(a, word, report)) {}
+    __device__ __forceinline__ Work(const PrefixArgs& a, uint32_t word, const Lens& len) {
         auto at = [&](uint32_t w) { return __shfl_sync(0xffffffffu, word, w); };
         part_row = static_cast<uint64_t>(at(1)) << 32 | at(0);
         tok0 = at(2), row0 = at(3), rows = at(4), kvh = at(5), ntok = at(6);
         pre_ref = at(7);
-        const uint32_t pre_blocks = at(8), pre_i = at(9), cap = at(10);
+        const uint32_t cap = at(10);
         suf_ref = at(11);
-        const uint32_t suf_blocks = at(12), suf_i = at(13), t0 = at(14), t1 = at(15);
+        const uint32_t t0 = at(14), t1 = at(15);
         flags = at(16);
         pair = rows > 128;
-        pre_len = __shfl_sync(0xffffffffu, page_len(a.prefix_lens, pre_i, pre_blocks, a.status, report), 0);
-        suf_len = __shfl_sync(0xffffffffu, page_len(a.suffix_lens, suf_i, suf_blocks, a.status, report), 0);
+        pre_len = __shfl_sync(0xffffffffu, len.pre, 0);
+        suf_len = __shfl_sync(0xffffffffu, len.suf, 0);
         // own tokens below the largest limit of the tile's rows
         const uint32_t top = limit((row0 + rows - 1) / a.G);
         const uint32_t p1 = min(t1, (pre_len + kTileTokens - 1) / kTileTokens);
@@ -305,6 +317,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t i0 = a.tc_ptr[blockIdx.x], i1 = a.tc_ptr[blockIdx.x + 1];
     launch_dependents();
+    uint32_t word = Work::fetch(a, i0, i1, lane);  // the next item's record
 
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
@@ -334,7 +347,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
-    uint32_t word = Work::fetch(a, i0, i1, lane);  // the next item's record
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -504,22 +516,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         const uint32_t ch = lane % kChunks, sub = lane / kChunks;
         uint32_t k = 0;  // tiles so far
         bool ok = true;
+        // The lengths and this thread's query token of the next item are loaded
+        // while the one before ends (its start took 900 clocks for the lengths and
+        // 2900 to the query rows in shared memory).
+        Work::Lens len;
+        uint32_t tok, row_j, row_h;  // token, query of the list, head of the group
+        auto ahead = [&] {
+            auto at = [&](uint32_t x) { return __shfl_sync(0xffffffffu, word, x); };
+            len = Work::lens(a, word, false);
+            const uint32_t tok0 = at(2), rows = at(4), rr = at(3) + (rows > 128 ? h * 128 : 0) + r;
+            row_j = rr / a.G;
+            row_h = rr - row_j * a.G;
+            tok = rr - at(3) < rows ? a.row_tok[tok0 + row_j] : 0u;
+        };
+        ahead();
         for (uint32_t i = i0; i < i1 && ok; ++i) {
-            const Work w(a, word, false);
+            const Work w(a, word, len);
             word = Work::fetch(a, i + 1, i1, lane);
             const uint32_t rbase = w.pair ? h * 128 : 0;
             const uint32_t mine = w.rows > rbase ? min(128u, w.rows - rbase) : 0;  // rows of this half
             const uint32_t cnt = w.count(h);
             const bool has = r < mine;
             const bool idle = lanes >= mine;  // no row of this warp
-            uint32_t at = 0;                  // this thread's row of q and out
-            int32_t lim_pre = 0, lim_suf = 0;
-            if (has) {
-                const uint32_t rr = w.row0 + rbase + r, j = rr / a.G;
-                at = a.row_tok[w.tok0 + j] * a.Hq + w.kvh * a.G + (rr - j * a.G);
-                lim_pre = static_cast<int32_t>(w.pre_len);
-                lim_suf = static_cast<int32_t>(w.limit(j));
-            }
+            // this thread's row of q and out
+            const uint32_t at = has ? tok * a.Hq + w.kvh * a.G + row_h : 0u;
+            const int32_t lim_pre = has ? static_cast<int32_t>(w.pre_len) : 0;
+            const int32_t lim_suf = has ? static_cast<int32_t>(w.limit(row_j)) : 0;
             if (cnt) {
 #pragma unroll 1
                 for (uint32_t y = sub; y < 32; y += kStep) {
@@ -527,6 +549,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                     cp_async16_zfill(qh + (ch >> 3) * 16384 + swz128(lanes + y, ch & 7), a.q + row * D + ch * 8,
                                      lanes + y < mine && a.scale != 0.0f);
                 }
+            }
+            // Pages beyond the pool: looked for once per item, while the query rows
+            // are on their way (a look at every tile took 130 clocks of it; one that
+            // waited for each 8 tiles 4700 of an item of 28), and tile by tile only
+            // where there are any.
+            bool beyond = false;
+#pragma unroll 4
+            for (uint32_t t = 0; t < w.n; t += 32 / kTilePages) {
+                const uint32_t tl = t + lane / kTilePages, pg = lane % kTilePages;
+                const bool in = tl < w.n && w.first(tl) + pg * kBlock < w.length(tl);
+                const uint32_t ref = in ? w.refs(a, tl)[pg] & kRefMask : 0u;
+                beyond |= in & (ref >= a.pool_blocks);
+            }
+            if (cnt) {
                 cp_async_wait_all();
                 if (a.scale < 0.0f) {  // a negative scale goes into Q: each lane flips what it copied
 #pragma unroll 1
@@ -538,16 +574,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 fence_proxy_async_shared();
                 mbar_arrive(&bars.q_full[h]);
             }
+            const bool any_bad = __any_sync(0xffffffffu, beyond);
             float m = -INFINITY, l = 0.0f;
-            // Pages beyond the pool: looked for once per item (a look at every tile
-            // took 130 clocks of it), and tile by tile only where there are any.
-            bool any_bad = false;
-#pragma unroll 1
-            for (uint32_t t = 0; t < w.n; t += 32 / kTilePages) {
-                const uint32_t tl = t + lane / kTilePages, pg = lane % kTilePages;
-                const bool in = tl < w.n && w.first(tl) + pg * kBlock < w.length(tl);
-                any_bad |= __any_sync(0xffffffffu, in && (w.refs(a, tl)[in ? pg : 0] & kRefMask) >= a.pool_blocks);
-            }
             // Tokens of the tile that this row sees, and that the warp's first row sees:
             // the rows' limits rise with the row, so the first one says whether any row
             // needs the mask.  They fall by a tile's tokens from tile to tile.
@@ -639,6 +667,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
                 if (t >= w.n_pre && t < w.n_pre + step) enter();
             }
             if (!ok) break;
+            ahead();
             // ---- this half's result
             if (cnt) {
                 if (!(ok = row_wait(&bars.o_done[h][(k - 1) & 1], ((k - 1) >> 1) & 1, a.status, 58))) break;
