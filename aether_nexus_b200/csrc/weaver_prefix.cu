@@ -300,9 +300,13 @@ constexpr uint64_t kStart16 = 6;
 static uint64_t rows16_item(const std::vector<uint64_t>& tiles, uint64_t slots) {
     uint64_t longest = 1, total = 0;
     for (uint64_t n : tiles) longest = std::max(longest, n), total += n;
-    uint64_t best = 4, least = ~0ull;
-    // no shorter than four waves of equal items, then in steps of an eighth
-    for (uint64_t per = std::max<uint64_t>(4, total / (4 * slots) / 4 * 4);; per += std::max<uint64_t>(4, per / 8 / 4 * 4)) {
+    // no shorter than four waves of equal items, then in steps of a quarter; with
+    // many tiles that shortest length already spreads them evenly (and the search
+    // would take the host long)
+    const uint64_t shortest = std::max<uint64_t>(4, total / (4 * slots) / 4 * 4);
+    if (tiles.size() > 8 * slots) return shortest;
+    uint64_t best = shortest, least = ~0ull;
+    for (uint64_t per = shortest;; per += std::max<uint64_t>(4, per / 4 / 4 * 4)) {
         std::vector<uint64_t> cost;
         for (uint64_t n : tiles) {
             const uint64_t k = (n + per - 1) / per;
