@@ -267,6 +267,44 @@ def test_bad_refs_are_skipped_and_reported(engine, rows):
     b.check()
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+def test_bad_refs_far_into_a_long_prefix(engine, rows):
+    """Many token tiles an item: single bad references at its start, middle and end."""
+    import torch
+    n = 40000
+    b = Batch([(n, [(rows, 20)])], 8, 8, 128, seed=19, junk=0.0)
+    refs, keep = list(b.prefix_refs), torch.ones(n, dtype=torch.bool, device="cuda")
+    for page in (0, 77, 1203, 1250, 2001, len(refs) - 1):
+        refs[page] = b.blocks + page
+        keep[page * 16:page * 16 + 16] = False
+    plan = b.plan(engine)
+    plan.run(**b.views(prefix_refs=Batch.words(refs)))
+    with pytest.raises(W.WeaverError) as e:
+        plan.status()
+    assert e.value.status == 4
+    b.prefix_rows = [b.prefix_rows[0][keep]]
+    b.check()
+
+
+@pytest.mark.parametrize("geometry", [(32, 8, 128), (14, 2, 64)], ids=lambda g: "x".join(map(str, g)))
+def test_own_lists_of_very_different_lengths(engine, geometry):
+    """Few rows a list, 1 to 6000 own tokens: items of many lengths, cut anywhere."""
+    b = Batch([(90, [(1, 1 + (i * 977) % 401 * (15 if i % 5 == 0 else 1)) for i in range(45)])], *geometry, seed=23)
+    plan = b.plan(engine)
+    plan.run(**b.views())
+    plan.status()
+    b.check()
+
+
+def test_more_lists_than_the_item_search_looks_at(engine):
+    """Thousands of short lists beside one long one."""
+    b = Batch([(40, [(1, 1 + i % 37) for i in range(470)] + [(1, 5000)])], 8, 8, 64, seed=29)
+    plan = b.plan(engine)
+    plan.run(**b.views())
+    plan.status()
+    b.check()
+
+
 def test_lengths_beyond_the_pages_are_cut_and_reported(engine):
     b = Batch([(32, [(1, 16)])], 4, 1, 64, seed=10)
     plan = b.plan(engine)
