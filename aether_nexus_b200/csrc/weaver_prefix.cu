@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(8 * D / 4) prefix_merge_kernel(const __grid_co
 constexpr uint32_t kOwnRows = 512;
 // Starting an item (query rows in, results out, the pipeline filling) in the
 // units of a token tile's cost: 16 sequences x 8 drafts run 34.9 us with 32, 35.1
-// with 40, 36.4 with 48, 36.9 with 56; 8 x 4 drafts 23.2, 24.6, 24.4 and 24.6.
+// with 40, 36.4 with 48, 36.9 with 56, 39.1 with 16; 8 x 4 drafts 22.9 to 24.6
+// with 32 to 56 and 26.5 with 16.
 constexpr uint32_t kItemCost = 32;
 // Lists of up to 16 rows go to the 16-row tiles, whose many small CTAs start
 // and end faster than items of the tensor-memory kernel; lists of 9 to 16 rows
