@@ -87,7 +87,9 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None 
 
         def pair_of(n):  # the (fractional) pair that turns n times
             return rot_dim * math.log(length / (n * 2.0 * math.pi)) / (2.0 * math.log(theta))
-        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim // 2 - 1)
+        # the ramp may end behind the last pair (the method bounds its end by rot_dim - 1): the last pairs
+        # then still turn more than `slow` times and are mixed, not scaled whole
+        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim - 1)
         ramp = np.clip((i - low) / max(high - low, 1e-3), 0.0, 1.0)
         factor = scaling.get("attention_factor")
         return f * (1.0 - ramp) + f / s * ramp, (0.1 * math.log(s) + 1.0) if factor is None else float(factor)

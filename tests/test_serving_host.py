@@ -45,6 +45,27 @@ def test_frequencies_yarn_and_bands_keep_fast_pairs_and_scale_slow_ones():
     assert ((h[mid] < f[mid]) & (h[mid] > f[mid] / 8.0)).all() and amp == 1.0
 
 
+@pytest.mark.parametrize("rot_dim,theta,length,factor", [
+    (128, 10000.0, 131072, 16.0), (128, 10000.0, 65536, 16.0), (16, 10000.0, 32768, 16.0), (64, 10000.0, 1 << 20, 4.0),
+    (128, 500000.0, 65536, 16.0)])
+def test_frequencies_yarn_ramp_may_end_behind_the_last_pair(rot_dim, theta, length, factor):
+    """The ramp between the pairs that turn 32 times and once over the original
+    length, written out pair by pair (Peng et al. 2023: its upper index is
+    bounded by rot_dim - 1, not by the last pair): a pair that still turns more
+    than once is mixed, never scaled whole."""
+    got, _ = W.rope_frequencies(rot_dim, theta, {"type": "yarn", "factor": factor, "original_length": length})
+
+    def index(turns):
+        return rot_dim / 2 * math.log(length / (2 * math.pi * turns)) / math.log(theta)
+    low, high = max(math.floor(index(32)), 0), min(math.ceil(index(1)), rot_dim - 1)
+    for i in range(rot_dim // 2):
+        f = theta ** (-2 * i / rot_dim)
+        inside = min(max((i - low) / (high - low), 0.0), 1.0)  # 0: keeps f, 1: f / factor
+        assert math.isclose(got[i], (1 - inside) * f + inside * f / factor, rel_tol=1e-12), i
+        if length * f / (2 * math.pi) > 1.0:
+            assert got[i] > f / factor * (1 + 1e-9), i
+
+
 @pytest.mark.parametrize("kw", [dict(rot_dim=7), dict(theta=-1.0), dict(theta=float("nan")),
                                 dict(scaling={"type": "other", "factor": 2.0}),
                                 dict(scaling={"type": "linear", "factor": 0.0}),
