@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <iterator>
 #include <memory>
 #include <new>
 #include <string>
@@ -1895,19 +1896,71 @@ bool disjoint_rows(uint64_t T, uint64_t H, uint64_t D, uint64_t ts, uint64_t hs)
     return heads_inside || tokens_inside;
 }
 
+// What an argument covers: [T][H] pieces of D bytes, token stride ts and head
+// stride hs in bytes.  A plain range is one piece.
+struct Rows {
+    const char* name;
+    const void* base;
+    uint64_t T, H, D, ts, hs;
+};
+Rows range(const char* name, const void* base, uint64_t bytes) { return Rows{name, base, base ? 1ull : 0ull, 1, bytes, 0, 0}; }
+
+// Whether two arguments may have bytes in common: not where their ranges are
+// apart, and not where both lie in separate residues of a common stride (slices
+// of one buffer of rows or heads).
+bool share(const Rows& x, const Rows& y) {
+    if (!x.T || !x.H || !x.D || !y.T || !y.H || !y.D) return false;
+    const uint64_t a = reinterpret_cast<uintptr_t>(x.base), b = reinterpret_cast<uintptr_t>(y.base);
+    auto span = [](const Rows& r) { return (r.T - 1) * r.ts + (r.H - 1) * r.hs + r.D; };
+    if (a + span(x) <= b || b + span(y) <= a) return false;
+    for (const uint64_t m : {x.T > 1 ? x.ts : 0, x.H > 1 ? x.hs : 0, y.T > 1 ? y.ts : 0, y.H > 1 ? y.hs : 0}) {
+        if (!m) continue;
+        // the residues start at base % m and are this many, if no more than m
+        auto residues = [m](const Rows& r) { return (r.ts % m ? (r.T - 1) * r.ts : 0) + (r.hs % m ? (r.H - 1) * r.hs : 0) + r.D; };
+        const uint64_t nx = residues(x), ny = residues(y), d = b >= a ? (b - a) % m : (m - (a - b) % m) % m;
+        if (nx <= d && ny <= m - d) return false;
+    }
+    return true;
+}
+
 int rope_output(const char* name, const void* in, uint64_t in_ts, uint64_t in_hs, const void* out, uint64_t ts,
                 uint64_t hs, uint64_t T, uint64_t H, uint64_t D) {
     if (!in || !out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s or its output is null", name);
     if (!aligned16(in) || !aligned16(out) || (T > 1 && (in_ts % 8 || ts % 8)) || (H > 1 && (in_hs % 8 || hs % 8)))
         return fail(WEAVER_ERR_MISALIGNED, "%s rows not 16-byte aligned", name);
     if (!disjoint_rows(T, H, D, ts, hs)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "rows of %s's output overlap", name);
-    const char* i0 = static_cast<const char*>(in);
-    const char* o0 = static_cast<const char*>(out);
-    if (T && H && !(in == out && (T == 1 || in_ts == ts) && (H == 1 || in_hs == hs))) {  // the same rows, or none in common
-        const char* i1 = i0 + 2 * ((T - 1) * in_ts + (H - 1) * in_hs + D);
-        const char* o1 = o0 + 2 * ((T - 1) * ts + (H - 1) * hs + D);
-        if (i0 < o1 && o0 < i1)
-            return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s's output overlaps it with other strides", name);
+    return WEAVER_OK;
+}
+
+// Warps read other tokens and heads while one of them writes: an output shares no
+// memory with any other argument, but for q_out and k_out over the same rows of
+// q and k, which each thread reads before it writes.
+int rope_overlaps(const weaver_rope_views* v, uint64_t D, bool append) {
+    const uint64_t T = v->n_tokens, Hq = v->q_heads, Hkv = v->kv_heads, w = 2 * D;
+    auto heads = [&](const char* name, const void* p, uint64_t H, uint64_t ts, uint64_t hs) {
+        return Rows{name, p, p ? T : 0, H, w, T > 1 ? 2 * ts : 0, H > 1 ? 2 * hs : 0};
+    };
+    const uint64_t pool = v->hot_pool_blocks * kBlock * Hkv * w;
+    const Rows ins[] = {heads("q", v->q, Hq, v->q_token_stride, v->q_head_stride),
+                        heads("k", v->k, Hkv, v->k_token_stride, v->k_head_stride),
+                        heads("v", append ? v->v : nullptr, Hkv, v->v_token_stride, v->v_head_stride),
+                        range("positions", v->positions, T * 4),
+                        range("q_weight", Hq ? v->q_weight : nullptr, w),
+                        range("k_weight", Hkv ? v->k_weight : nullptr, w),
+                        range("slots", append ? v->slots : nullptr, T * 8)};
+    const Rows outs[] = {heads("q_out", v->q_out, Hq, v->q_out_token_stride, v->q_out_head_stride),
+                         heads("k_out", append ? nullptr : v->k_out, Hkv, v->k_out_token_stride, v->k_out_head_stride),
+                         range("hot_k", append ? v->hot_k : nullptr, pool), range("hot_v", append ? v->hot_v : nullptr, pool),
+                         range("bad_flag", append ? v->bad_flag : nullptr, 4)};
+    for (size_t o = 0; o < std::size(outs); ++o) {
+        const Rows& x = outs[o];
+        for (size_t i = 0; i < std::size(ins); ++i) {
+            const Rows& y = ins[i];
+            if (i == o && o < 2 && x.base == y.base && x.ts == y.ts && x.hs == y.hs) continue;  // in place
+            if (share(x, y)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s overlaps %s", x.name, y.name);
+        }
+        for (size_t i = 0; i < o; ++i)
+            if (share(x, outs[i])) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s overlaps %s", x.name, outs[i].name);
     }
     return WEAVER_OK;
 }
@@ -1949,6 +2002,7 @@ int rope_run(weaver_rope* rope, const weaver_rope_views* v, void* stream, bool a
                                                 v->k_out_token_stride, v->k_out_head_stride, T, v->kv_heads, D))) {
         return rc;
     }
+    if ((rc = rope_overlaps(v, D, append))) return rc;
     a.q = v->q;
     a.k = v->k;
     a.v = append ? v->v : nullptr;

@@ -210,7 +210,8 @@ class Rope:
         """``q_out`` / ``k_out`` = the rotated (with a weight: normed, then
         rotated) ``q [T, Hq, d]`` / ``k [T, Hkv, d]`` (float16 or bfloat16, any
         token and head strides; outputs of the inputs' type, the input itself
-        included).  ``q`` or ``k`` may be None.  ``positions [T]`` int32."""
+        included, but no memory of another argument).  ``q`` or ``k`` may be
+        None.  ``positions [T]`` int32."""
         T, hq, hkv, dt, qv, kv, qo, pos, qw, kw = self._inputs(q, k, positions, q_weight, k_weight, q_out, None)
         ko = (0, 0, 0) if k is None else self._heads("k_out", k_out, (T, hkv, self.head_dim), dt)
         raw = _VIEWS(T, hq, hkv, self._types[dt], qv[0], kv[0], 0, qv[1], qv[2], kv[1], kv[2], 0, 0, pos, qw, kw, eps, 0,
@@ -226,7 +227,9 @@ class Rope:
         None.  ``hot_k`` / ``hot_v`` may be raw device pointers (a
         ``DeviceFabric`` layer's) with ``hot_pool_blocks``.  ``bad_flag`` (one
         int32) gets 1 OR-ed in for a slot beyond the pool, whose token is
-        skipped.  The slots of one call must be distinct."""
+        skipped.  The slots of one call must be distinct.  ``q_out`` (``q``
+        itself excepted), the pools and ``bad_flag`` share no memory with another
+        argument."""
         if k is None:
             raise ValueError("append needs k")
         T, hq, hkv, dt, qv, kv, qo, pos, qw, kw = self._inputs(q, k, positions, q_weight, k_weight, q_out, self._f16)

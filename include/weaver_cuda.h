@@ -481,7 +481,11 @@ typedef struct weaver_rope_config {
 } weaver_rope_config;
 
 /* Strides are in elements, multiples of 8 (0 included for inputs, any value
- * where there is one token or head); a head's head_dim elements are contiguous.  All pointers 16-byte aligned device pointers. */
+ * where there is one token or head); a head's head_dim elements are contiguous.
+ * All pointers are device pointers, those of 16-bit elements 16-byte aligned.
+ * An output (q_out, k_out, the pools, bad_flag) shares no memory with another
+ * argument, q_out == q and k_out == k with the same strides excepted; slices of
+ * one buffer that lie next to each other in every row or head are apart. */
 typedef struct weaver_rope_views {
     uint32_t n_tokens, q_heads, kv_heads;
     uint32_t dtype;            /* weaver_dtype of q, k, v and the weights */

@@ -290,3 +290,35 @@ def test_no_tokens(engine):
     none = torch.empty(0, dtype=torch.int32, device="cuda")
     rope.rotate(e, e, none, e, e)
     rope.append(e, e, None, none, none.long(), pool, None, e, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("layout", ["tokens", "heads", "pairs"])
+def test_slices_of_one_buffer_lie_next_to_each_other(engine, layout):
+    """Inputs and outputs that share a buffer and no element of it: the same results as from buffers of their own."""
+    import torch
+    T, H, d = 37, 4, 64
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) + 11
+    rope = W.Rope(engine, head_dim=d)
+    data = [heads(T, H, d, torch.float16, 50 + i) for i in range(4)]
+    if layout == "tokens":    # [T][q k q_out k_out][H][d]
+        buf = torch.zeros(T, 4, H, d, dtype=torch.float16, device="cuda")
+        part = [buf[:, i] for i in range(4)]
+    elif layout == "heads":   # [q k q_out k_out][H][T][d], one after the other
+        buf = torch.zeros(4, H, T, d, dtype=torch.float16, device="cuda")
+        part = [buf[i].transpose(0, 1) for i in range(4)]
+    else:                     # [T][H][q k q_out k_out][d]
+        buf = torch.zeros(T, H, 4, d, dtype=torch.float16, device="cuda")
+        part = [buf[:, :, i] for i in range(4)]
+    for p, x in zip(part, data):
+        p.copy_(x)
+    rope.rotate(part[0], part[1], pos, part[2], part[3])
+    for i in range(2):
+        assert torch.equal(part[i], data[i])
+        check(part[2 + i], *reference(data[i], pos, rope.inv_freq, 1.0, d, "half"))
+    before = buf.clone()
+    for args in ((part[0], part[1], part[1], part[3]), (part[0], part[1], part[2], part[2]),
+                 (part[0], part[1], part[2], part[0])):
+        with pytest.raises(W.WeaverError) as e:
+            rope.rotate(args[0], args[1], pos, args[2], args[3])
+        assert e.value.status == 1
+    assert torch.equal(buf, before)

@@ -156,6 +156,41 @@ def test_append_refuses(engine_memory, kw, status):
     N.lib().weaver_rope_destroy(h)
 
 
+# q covers 8192 bytes from 1 << 20, k and v 2048 each from 2 << 20 and 3 << 20 (two heads of 256 bytes a token)
+OVERLAPS = [
+    dict(q_out=2 << 20, q_heads=2, q_token_stride=256, q_out_token_stride=256),   # k itself
+    dict(q_out=(2 << 20) - 8192 + 256),                                           # its last head: k's first
+    dict(q_out=(4 << 20) - 4096), dict(q_out=(11 << 20) - 4096, q_weight=11 << 20), dict(q_out=11 << 20, k_weight=11 << 20),
+]
+
+
+@pytest.mark.parametrize("kw", OVERLAPS + [
+    dict(k_out=1 << 20), dict(k_out=(1 << 20) + 8192 - 256), dict(k_out=4 << 20), dict(k_out=5 << 20),
+    dict(k_out=(5 << 20) + 1024, k_out_token_stride=1024),                        # two of the heads of q_out
+    dict(k=5 << 20, k_out=5 << 20), dict(k=1 << 20, q_out=1 << 20)])              # in place over what another one reads
+def test_rotate_refuses_outputs_over_other_arguments(engine_memory, kw):
+    rc, h = _rope(engine_memory)
+    assert rc == 0
+    assert N.lib().weaver_rope_rotate(h, ctypes.byref(_rope_views(**kw)), None) == INVALID, N.lib().weaver_last_error()
+    assert b"overlap" in N.lib().weaver_last_error()
+    N.lib().weaver_rope_destroy(h)
+
+
+# the pools cover 32768 bytes from 8 << 20 and 9 << 20
+@pytest.mark.parametrize("kw", OVERLAPS + [
+    dict(q_out=3 << 20), dict(q_out=8 << 20), dict(q_out=(9 << 20) + 32768 - 256), dict(q_out=(8 << 20) - 4096),
+    dict(q_out=7 << 20), dict(q_out=(10 << 20) - 4096),
+    dict(q=8 << 20), dict(k=8 << 20), dict(k=(8 << 20) + 32768 - 256), dict(v=9 << 20), dict(v=8 << 20), dict(k=9 << 20),
+    dict(slots=(8 << 20) + 32768 - 8), dict(positions=9 << 20), dict(bad_flag=9 << 20), dict(k_weight=8 << 20),
+    dict(bad_flag=(7 << 20) + 8), dict(bad_flag=4 << 20), dict(bad_flag=(1 << 20) + 4)])
+def test_append_refuses_outputs_over_other_arguments(engine_memory, kw):
+    rc, h = _rope(engine_memory)
+    assert rc == 0
+    assert N.lib().weaver_rope_append(h, ctypes.byref(_rope_views(**kw)), None) == INVALID, N.lib().weaver_last_error()
+    assert b"overlap" in N.lib().weaver_last_error()
+    N.lib().weaver_rope_destroy(h)
+
+
 def test_no_tokens_is_no_launch(engine_memory):
     rc, h = _rope(engine_memory)
     empty = N.RopeViewsC()
