@@ -2209,8 +2209,6 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
     } else {
         if (!v->out) return fail(WEAVER_ERR_INVALID_ARGUMENT, "views.out is null");
         if (!aligned16(v->out)) return fail(WEAVER_ERR_MISALIGNED, "out not 16-byte aligned");
-        if (v->q && overlap(v->q, v->out, static_cast<uint64_t>(a.n_tokens) * a.Hq * a.D * 2))
-            return fail(WEAVER_ERR_INVALID_ARGUMENT, "out overlaps q");
         a.out = static_cast<__half*>(v->out);
     }
     if (plan->n_prefix_pages + plan->n_suffix_pages) {
@@ -2224,6 +2222,25 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
         for (const void* p : {static_cast<const void*>(v->prefix_refs), static_cast<const void*>(v->suffix_refs),
                               static_cast<const void*>(v->prefix_lens), static_cast<const void*>(v->suffix_lens)})
             if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(WEAVER_ERR_MISALIGNED, "block refs or lengths misaligned");
+    }
+    {   // items write their rows while others still read
+        const uint64_t rows = static_cast<uint64_t>(a.n_tokens) * a.Hq, pre = plan->n_prefix_pages, suf = plan->n_suffix_pages;
+        const uint64_t pool = pre + suf ? v->hot_pool_blocks * kBlock * a.Hkv * a.D * 2 : 0;
+        const Rows ins[] = {range("q", v->q, rows * a.D * 2),
+                            range("hot_k", v->hot_k, pool),
+                            range("hot_v", v->hot_v, pool),
+                            range("prefix_refs", v->prefix_refs, pre * 4),
+                            range("suffix_refs", v->suffix_refs, suf * 4),
+                            range("prefix_lens", v->prefix_lens, pre ? plan->shape.num_groups * 4ull : 0),
+                            range("suffix_lens", v->suffix_lens, suf ? plan->shape.num_seqs * 4ull : 0)};
+        const Rows outs[] = {range("out", a.out, rows * a.D * 2), range("part_m", a.out_m, rows * 4),
+                             range("part_l", a.out_l, rows * 4), range("part_o", a.out_o, rows * a.D * 4)};
+        for (size_t o = 0; o < std::size(outs); ++o) {
+            for (const Rows& in : ins)
+                if (share(outs[o], in)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s overlaps %s", outs[o].name, in.name);
+            for (size_t i = 0; i < o; ++i)
+                if (share(outs[o], outs[i])) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s overlaps %s", outs[o].name, outs[i].name);
+        }
     }
     a.q = static_cast<const __half*>(v->q);
     a.k = static_cast<const __half*>(v->hot_k);

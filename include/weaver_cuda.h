@@ -536,12 +536,12 @@ WEAVER_EXPORT int weaver_rope_append(weaver_rope* rope, const weaver_rope_views*
  * One token per sequence, draft batches and prompt chunks may be mixed; a
  * group of one sequence with no prefix is a plain paged sequence.
  *
- * Rows of q and out behind the last query are not touched; out and q do not
- * overlap; the lengths and references stay as they are while a run is in
- * flight.  The tokens of the last page past a length, and pages past it, are not
- * part of the result whatever the pool holds there.  A NaN or infinite value at a
- * position that some query of a call sees can turn the outputs of other
- * queries of that head NaN too, causally masked or not.
+ * Rows of q and out behind the last query are not touched; the outputs share no
+ * memory with an input or with each other; the lengths and references stay as
+ * they are while a run is in flight.  The tokens of the last page past a length,
+ * and pages past it, are not part of the result whatever the pool holds there.
+ * A NaN or infinite value at a position that some query of a call sees can turn
+ * the outputs of other queries of that head NaN too, causally masked or not.
  * WEAVER_FLAG_PARTIALS writes (m, l, o) instead of out, as weaver_run does, so
  * that a plan over cold blocks of the same queries can be merged with
  * weaver_merge_partials. */

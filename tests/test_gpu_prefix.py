@@ -438,3 +438,50 @@ def test_negative_and_zero_scale(engine):
     plan.status()
     small.q = -small.q
     small.check()
+
+
+@pytest.mark.parametrize("over", ["q", "q_last_row", "hot_k", "hot_v_last_page", "prefix_refs", "suffix_refs", "prefix_lens",
+                                  "suffix_lens"])
+@pytest.mark.parametrize("partials", [False, True])
+def test_outputs_over_inputs_are_refused(engine, over, partials):
+    """Every output over every input, by whole buffers and by a last row; nothing is written."""
+    import torch
+    b = Batch([(32, [(2, 16), (1, 3)])], 4, 1, 64, seed=21, junk=0.0)
+    plan = b.plan(engine, partials=partials)
+    views = b.views()
+    for name in ("q", "hot_k", "hot_v", "prefix_refs", "suffix_refs", "prefix_lens", "suffix_lens"):
+        # behind each input as much room as the largest output takes
+        t = views[name]
+        room = torch.zeros(t.numel() * t.element_size() + 16384, dtype=torch.uint8, device="cuda")
+        views[name] = room[:t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+        views[name].copy_(t)
+    name = over.split("_last")[0]
+    t = views[name]
+    at = t.data_ptr() + (t.numel() * t.element_size() - 16 if "_last" in over else 0)
+    assert at % 16 == 0
+    n = b.T * b.Hq
+    own = dict(part_m=torch.zeros(n, device="cuda"), part_l=torch.zeros(n, device="cuda"),
+               part_o=torch.zeros(n, b.d, device="cuda"), out=None) if partials else dict(out=b.out)
+    held = t.clone()
+    for output in [x for x, y in own.items() if y is not None]:
+        with pytest.raises(W.WeaverError) as e:
+            plan.run(**{**views, **own, output: at})
+        assert e.value.status == 1 and "overlaps " + name in str(e.value)
+    assert torch.equal(t, held)
+    plan.run(**{**views, **own})
+    plan.status()
+
+
+def test_partial_outputs_over_each_other_are_refused(engine):
+    import torch
+    b = Batch([(32, [(2, 16), (1, 3)])], 4, 1, 64, seed=22)
+    plan = b.plan(engine, partials=True)
+    n = b.T * b.Hq
+    room = torch.zeros(n * (b.d + 2), device="cuda")
+    m, l, o = room[n * b.d:n * b.d + n], room[n * b.d + n:], room[:n * b.d]
+    plan.run(**b.views(out=None, part_m=m, part_l=l, part_o=o))  # neighbours
+    plan.status()
+    for args in ((m, m, o), (m, o[-n:], o), (o[:n], l, o), (room[n * b.d - 1:][:n], l, o), (m, room[n * b.d + n - 1:][:n], o)):
+        with pytest.raises(W.WeaverError) as e:
+            plan.run(**b.views(out=None, part_m=args[0], part_l=args[1], part_o=args[2]))
+        assert e.value.status == 1
