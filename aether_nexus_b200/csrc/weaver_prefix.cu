@@ -291,6 +291,14 @@ constexpr uint32_t kItemCost = 32;
 // us on tensor memory, 31 with both; 200 sequences x 3: 129 and 94).
 constexpr uint32_t kRows16 = 16, kRowsFew = 8;
 
+// The longest run of an item.  The tensor cores cut the bits below the
+// accumulator's last off where they add a step of 16 tokens to it, so O comes out
+// low by up to 2^-22 of itself a step, half of that over a run that grows evenly:
+// 1.4e-3 after 2^14 steps, more than the rounding of the result.  2048 steps leave
+// it below 2^-12; the runs are joined in fp32.  512 token tiles of four steps;
+// 8192 pages of one step, dealt to four warps.
+constexpr uint32_t kMostTiles = 512, kMostPages = 8192;
+
 // The length of a 16-row item, in pages: that of least makespan on `slots`
 // resident CTAs, where an item costs kStart16 rounds beside a round for every
 // four of its pages (a page per warp).  64 sequences behind one prefix, 38 MB of
@@ -446,7 +454,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
     std::vector<uint64_t> sizes;
     for (const PrefixTile& T : t->tiles)
         if (t->lists[T.list].tile_rows == 16) sizes.push_back(pages(T.list));
-    const uint64_t per = rows16_item(sizes, 3 * n_sm);
+    const uint64_t per = std::min<uint64_t>(rows16_item(sizes, 3 * n_sm), kMostPages);
     for (uint32_t ti = 0; ti < t->tiles.size(); ++ti) {
         PrefixTile& T = t->tiles[ti];
         if (t->lists[T.list].tile_rows != 16) continue;
@@ -488,7 +496,7 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
                 ++cta;
                 continue;
             }
-            take = std::min<uint64_t>(take, x.n - b);
+            take = std::min<uint64_t>({take, x.n - b, kMostTiles});
             PrefixItem it = item_of(T, kTcPages);
             it.part_row = part_rows + static_cast<uint64_t>(T.n_slots) * T.rows;
             it.t0 = b;

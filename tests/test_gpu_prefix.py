@@ -485,3 +485,58 @@ def test_partial_outputs_over_each_other_are_refused(engine):
         with pytest.raises(W.WeaverError) as e:
             plan.run(**b.views(out=None, part_m=args[0], part_l=args[1], part_o=args[2]))
         assert e.value.status == 1
+
+
+def one_list(kind, n, logits_of, sink=False):
+    """Lists of n tokens that share nine pages, so that the formula is a sum over
+    their 144 rows by how often they come: "prompt" is one sequence of 2048
+    queries (8192 rows a kv head), "single_tokens" 300 of one query; either way an
+    item walks through as much of a list as a plan gives it.  Only the first
+    dimension of q and K counts.  Returns (plan's arguments, tensors, out, the
+    rows' scores, their counts, v) with the last three in 64 bits."""
+    import torch
+    Hq, Hkv, d, kinds = 32, 8, 128, 9
+    g = torch.Generator(device="cuda").manual_seed(31)
+    logits = logits_of(torch.randn(kinds, 16, generator=g, device="cuda"))
+    hot_k = torch.zeros(kinds, 16, Hkv, d, dtype=torch.float16, device="cuda")
+    hot_v = torch.rand(kinds, 16, 1, d, generator=g, device="cuda").add_(0.5).half().repeat(1, 1, Hkv, 1)
+    if sink:
+        logits[0, 0] = 0.0
+        hot_v[0, 0] = 0.0
+    hot_k[..., 0] = (logits / (8.0 * d ** -0.5)).half()[..., None]
+    pages = [0] + [1 + i % (kinds - 1) for i in range(n // 16 - 1)]
+    seqs = 1 if kind == "prompt" else 300
+    nq = 2048 if kind == "prompt" else 1
+    q = torch.zeros(seqs * nq, Hq, d, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0
+    out = torch.full_like(q, math.nan)
+    geometry = dict(q_heads=Hq, kv_heads=Hkv, head_dim=d, scale=d ** -0.5, q_indptr=[nq * b for b in range(seqs + 1)],
+                    suffix_indptr=[len(pages) * b for b in range(seqs + 1)], causal=False)
+    tensors = dict(q=q, hot_k=hot_k, hot_v=hot_v, suffix_refs=Batch.words(pages * seqs), out=out)
+    count = torch.bincount(torch.tensor(pages, device="cuda"), minlength=kinds).double()[:, None]
+    return geometry, tensors, out, hot_k[:, :, 0, 0].double() * 8.0 * d ** -0.5, count, hot_v[:, :, 0].double()
+
+
+@pytest.mark.parametrize("kind,n", [("prompt", 1 << 19), ("single_tokens", 1 << 20)])
+def test_long_sums_do_not_drift(engine, kind, n):
+    """Flat scores over a very long list.
+
+    The tensor cores add 16 tokens a step to the accumulator in two sums that are
+    cut, not rounded: at most 2 * 2^-23 of it a step, so 2^-23 a step of the final
+    sum while it grows evenly, 2^-12 over the 2048 steps of the longest run.  The
+    fp32 sum of the probabilities is off by 2^-24 for each of the run's additions,
+    512 of a token tile or 2048 of a page: 2^-13.  Both times W, beside the
+    module's bound."""
+    import torch
+    geometry, tensors, out, s, count, v = one_list(kind, n, lambda x: x)
+    plan = W.PrefixPlan(engine, **geometry)
+    plan.run(**tensors)
+    plan.status()
+    p = torch.exp(s - s.max()) * count
+    l = p.sum()
+    y = (p[..., None] * v).sum((0, 1)) / l  # v > 0: also W
+    ds = (128 + 4) * 2.0 ** -24 * s.abs().amax()
+    tol = y * (2.0 ** -11 + 2.0 ** -11 + 2 * ds + 2.0 ** -17 + 2.0 ** -12 + 2.0 ** -13) + n * 2.0 ** -25 * v.amax() / l + \
+        2.0 ** -25
+    err = (out.double() - y).abs()
+    assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f}, {float((err / y).max()):.5f} of the value"
