@@ -39,8 +39,10 @@ __device__ __forceinline__ void fa_load_q(const __half* qs, uint32_t qf[D / 16][
 // One block: scores (times `scale`), positions pos0 + t masked at or past the
 // row's limit lim[hh] (and all of them when !valid), online softmax update of
 // (m_run, l_run) per row, O += P V.  l_run is this lane's partial sum (the
-// caller adds the quad's lanes at the end).
-template <int D>
+// caller adds the quad's lanes at the end).  Both l_run and O come times
+// 2^kShift: with a shift of up to 15 probabilities far below the maximum keep
+// their bits in f16, whose least step is 2^-24.
+template <int D, int kShift = 0>
 __device__ __forceinline__ void fa_block(const uint8_t* Ks, const uint8_t* Vs, const uint32_t qf[D / 16][4],
                                          const int32_t lim[2], int32_t pos0, float scale, bool valid,
                                          float m_run[2], float l_run[2], float o[D / 8][4], uint32_t lane) {
@@ -78,7 +80,10 @@ __device__ __forceinline__ void fa_block(const uint8_t* Ks, const uint8_t* Vs, c
         const float m_new = fmaxf(m_run[hh], mx);
         const float alpha = exp_shift(m_run[hh], m_new);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pv[hh][e] = exp_shift(sv[e], m_new);
+        for (int e = 0; e < 4; ++e) {
+            pv[hh][e] = exp_shift(sv[e], m_new);
+            if (kShift) pv[hh][e] *= static_cast<float>(1 << kShift);
+        }
         l_run[hh] = l_run[hh] * alpha + (pv[hh][0] + pv[hh][1]) + (pv[hh][2] + pv[hh][3]);
         m_run[hh] = m_new;
 #pragma unroll

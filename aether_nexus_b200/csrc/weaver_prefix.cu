@@ -39,6 +39,10 @@ namespace weaver {
 namespace {
 
 constexpr uint32_t kPxThreads = 128;
+// log2 of the factor on the probabilities: the largest is 2^15, inside f16, and
+// what f16 cannot hold any more is 2^-40 of it (at 1 a long tail 2^-25 below one
+// dominant token vanished from the output while the sum counted it)
+constexpr int kPxShift = 15;
 
 template <int D>
 struct PxLayout {
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const __grid_
             __syncwarp();
             const uint8_t* Ks = ring + (stage++ & 1) * L::kStage;
             const bool o_own = __shfl_sync(0xffffffffu, own, i);
-            fa_block<D>(Ks, Ks + L::kTile, qf, o_own ? lim_suf : lim_pre,
+            fa_block<D, kPxShift>(Ks, Ks + L::kTile, qf, o_own ? lim_suf : lim_pre,
                         static_cast<int32_t>(__shfl_sync(0xffffffffu, pos, i)), a.scale, true, m_run, l_run, o, lane);
             __syncwarp();  // every lane done with the stage before it is refilled
         }
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kPxThreads) prefix_rows16_kernel(const __grid_
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             float* pw = red + (w * 16 + tid) * (D + 2);
-            const float f = exp_shift(pw[0], M);
+            const float f = exp_shift(pw[0], M) * (1.0f / (1 << kPxShift));
             Lsum += pw[1] * f;
             pw[0] = f;
         }

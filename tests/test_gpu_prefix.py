@@ -540,3 +540,31 @@ def test_long_sums_do_not_drift(engine, kind, n):
         2.0 ** -25
     err = (out.double() - y).abs()
     assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f}, {float((err / y).max()):.5f} of the value"
+
+
+@pytest.mark.parametrize("tail,spread", [(-14.0, 1.0), (-17.5, 0.0), (-20.0, 1.0)])
+@pytest.mark.parametrize("kind,n", [("prompt", 1 << 18), ("single_tokens", 1 << 14)])
+def test_one_dominant_token_leaves_the_tail_its_weight(engine, kind, n, tail, spread):
+    """A first token that takes nearly all of the softmax and has V = 0 (an
+    attention sink) before a long tail `tail` nats below it: the output is the
+    tail's share.
+
+    The probabilities are held in f16 times a power of two, at least 2^7 for the
+    largest, so one below f16's normal numbers is off by at most 2^-25 against a
+    sum of 2^7: n 2^-32 max|v| in all.  Beside it the relative terms of the
+    module's bound and of long sums (test_long_sums_do_not_drift), times W, here
+    the tail's own share."""
+    import torch
+    geometry, tensors, out, s, count, v = one_list(kind, n, lambda x: tail + spread * x, sink=True)
+    plan = W.PrefixPlan(engine, **geometry)
+    plan.run(**tensors)
+    plan.status()
+    p = torch.exp(s) * count
+    l = p.sum()
+    y = (p[..., None] * v).sum((0, 1)) / l
+    ds = (128 + 4) * 2.0 ** -24 * s.abs().amax()
+    tol = y * (2.0 ** -11 + 2.0 ** -11 + 2 * ds + 2.0 ** -17 + 2.0 ** -12 + 2.0 ** -13) + n * 2.0 ** -32 * v.amax() / l + \
+        2.0 ** -25
+    assert (tol < 0.25 * y).all()  # the bound says something about the tail
+    err = (out.double() - y).abs()
+    assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f}, {float((err / y).max()):.3f} of the value"
