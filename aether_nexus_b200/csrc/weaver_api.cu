@@ -2041,7 +2041,6 @@ struct weaver_prefix_plan {
     void* arena = nullptr;
     uint32_t n_items16 = 0, n_tc_ctas = 0, max_slots = 0;
     uint64_t n_prefix_pages = 0, n_suffix_pages = 0;
-    cudaStream_t last_stream = nullptr;
 };
 
 extern "C" {
@@ -2251,7 +2250,6 @@ int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* v, vo
     a.prefix_lens = v->prefix_lens;
     a.suffix_lens = v->suffix_lens;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    plan->last_stream = s;
     DeviceScope dev(plan->device);
     WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
     if (plan->n_items16) WEAVER_CUDA_TRY(launch_prefix_rows16(a, plan->n_items16, s), "prefix attention launch");
@@ -2270,10 +2268,15 @@ int weaver_prefix_plan_status(weaver_prefix_plan* plan) {
     if (!plan) return fail(WEAVER_ERR_INVALID_ARGUMENT, "null plan");
     DeviceScope dev(plan->device);
     WEAVER_CUDA_TRY(dev.err, "cudaSetDevice");
-    WEAVER_CUDA_TRY(cudaStreamSynchronize(plan->last_stream), "stream synchronize");
+    // the device, not a stream: a captured run is replayed on any stream, and the
+    // one that it was captured on may be gone
+    WEAVER_CUDA_TRY(cudaDeviceSynchronize(), "device synchronize");
     uint32_t st[2] = {0, 0};
     WEAVER_CUDA_TRY(cudaMemcpy(st, plan->base.status, sizeof(st), cudaMemcpyDeviceToHost), "status read");
-    if (st[0] || st[1]) WEAVER_CUDA_TRY(cudaMemset(plan->base.status, 0, sizeof(st)), "status reset");
+    if (st[0] || st[1]) {  // done before a run on a non-blocking stream can set it again
+        WEAVER_CUDA_TRY(cudaMemset(plan->base.status, 0, sizeof(st)), "status reset");
+        WEAVER_CUDA_TRY(cudaDeviceSynchronize(), "status reset");
+    }
     if (st[0] & DEVERR_TIMEOUT) return fail(WEAVER_ERR_TIMEOUT, "a device-side wait timed out (site %u)", st[1] & 0xFFu);
     if (st[0] & DEVERR_REF_RANGE)
         return fail(WEAVER_ERR_OUT_OF_RANGE, "a block reference was beyond the pool, or a length beyond its pages");

@@ -139,8 +139,9 @@ class PrefixPlan:
         self.run_views(self.views(**tensors), stream)
 
     def status(self) -> None:
-        """Synchronise and raise ``WeaverError`` if a run met a block reference
-        beyond the pool or a length beyond its pages."""
+        """Wait for the device's work, replayed graphs included, and raise
+        ``WeaverError`` if a run met a block reference beyond the pool or a
+        length beyond its pages."""
         N.check(N.lib().weaver_prefix_plan_status(self._h))
 
 

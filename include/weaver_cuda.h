@@ -585,10 +585,11 @@ WEAVER_EXPORT void weaver_prefix_plan_destroy(weaver_prefix_plan* plan);
 WEAVER_EXPORT int weaver_prefix_run(weaver_prefix_plan* plan, const weaver_prefix_views* views, void* stream);
 /* Number of kernels one weaver_prefix_run launches. */
 WEAVER_EXPORT int weaver_prefix_plan_kernel_count(const weaver_prefix_plan* plan);
-/* Synchronises the plan's last stream, then reads and clears its status:
- * WEAVER_OK, WEAVER_ERR_OUT_OF_RANGE (a block ref beyond the pool, whose
- * tokens were skipped, or a length beyond its pages, which was cut) or
- * WEAVER_ERR_TIMEOUT. */
+/* Waits for all work of the plan's device (replayed graphs on any stream
+ * included; so not while a stream of the process captures), then reads and
+ * clears the plan's status: WEAVER_OK, WEAVER_ERR_OUT_OF_RANGE (a block ref
+ * beyond the pool, whose tokens were skipped, or a length beyond its pages,
+ * which was cut) or WEAVER_ERR_TIMEOUT. */
 WEAVER_EXPORT int weaver_prefix_plan_status(weaver_prefix_plan* plan);
 
 /* ---- self-test of the bounded device-side waits --------------------------

@@ -568,3 +568,34 @@ def test_one_dominant_token_leaves_the_tail_its_weight(engine, kind, n, tail, sp
     assert (tol < 0.25 * y).all()  # the bound says something about the tail
     err = (out.double() - y).abs()
     assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f}, {float((err / y).max()):.3f} of the value"
+
+
+def test_status_waits_for_a_replay_on_another_stream(engine):
+    """A captured run replayed behind other work, not on the stream it was
+    captured on: the status that follows at once is that run's, and it is cleared
+    for the next."""
+    import torch
+    b = Batch([(300, [(2, 20)])], 4, 1, 128, seed=33, junk=0.0)
+    refs, good = Batch.words(b.prefix_refs), Batch.words(b.prefix_refs)
+    plan = b.plan(engine)
+    views = b.views(prefix_refs=refs)
+    torch.cuda.synchronize()
+    graph, side, other = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        plan.run(**views)
+    for bad in (True, False, True):
+        refs.copy_(good)
+        if bad:
+            refs[3] = b.blocks
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            graph.replay()
+        if bad:
+            with pytest.raises(W.WeaverError) as e:
+                plan.status()
+            assert e.value.status == 4
+        else:
+            plan.status()
+            b.check()
+        assert other.query()
