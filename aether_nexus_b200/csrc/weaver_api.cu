@@ -2149,6 +2149,9 @@ int weaver_prefix_plan_create(weaver_engine* eng, const weaver_prefix_shape* sh,
     if (e != cudaSuccess) return cuda_fail(e, "prefix plan allocation");
     char* base = static_cast<char*>(plan->arena);
     e = cudaMemcpy(base, image.data(), image.size(), cudaMemcpyHostToDevice);
+    // a copy from pageable memory may return before its last part has landed, and a
+    // run on a non-blocking stream does not wait for the stream that it is on
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
         cudaFree(plan->arena);
         return cuda_fail(e, "prefix plan upload");

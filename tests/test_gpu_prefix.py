@@ -599,3 +599,29 @@ def test_status_waits_for_a_replay_on_another_stream(engine):
             plan.status()
             b.check()
         assert other.query()
+
+
+def test_a_plan_is_ready_when_it_is_made(engine):
+    """Plans of different batches made, run at once on a stream of their own and
+    dropped, one after the other in the memory that the last one left."""
+    import torch
+    bs = [Batch(SHAPES[s], 8, 2, 128, seed=34 + i) for i, s in enumerate(("drafts", "prompts", "many_sequences"))]
+    views = [b.views(out=None) for b in bs]
+    want = []
+    for b in bs:
+        plan = b.plan(engine)
+        plan.run(**b.views())
+        plan.status()
+        b.check()
+        want.append(b.out.clone())
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(30):
+        b = bs[i % 3]
+        out = torch.empty_like(b.out)
+        torch.cuda.synchronize()
+        plan = b.plan(engine)
+        plan.run(stream, **{**views[i % 3], "out": out})
+        stream.synchronize()
+        assert torch.equal(out, want[i % 3])
+        plan.close()
