@@ -62,7 +62,7 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None 
     f = float(theta) ** (-2.0 * i / max(rot_dim, 1))
     if not scaling:
         return f, 1.0
-    kind, s = scaling.get("type"), float(scaling["factor"])
+    kind = scaling.get("type")
     known = {"linear": set(), "ntk": set(), "yarn": {"original_length", "beta_fast", "beta_slow", "attention_factor"},
              "bands": {"original_length", "low", "high"}}
     if kind not in known:
@@ -70,20 +70,29 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None 
     extra = set(scaling) - known[kind] - {"type", "factor"}
     if extra:
         raise ValueError(f"rope scaling {kind!r} does not take {sorted(extra)}")
-    if not (math.isfinite(s) and s > 0):
-        raise ValueError(f"rope scaling factor {s}")
+
+    def positive(name, default=None):
+        x = scaling.get(name, default)
+        if x is None:
+            raise ValueError(f"rope scaling {kind!r} needs {name}")
+        x = float(x)
+        if not (math.isfinite(x) and x > 0):
+            raise ValueError(f"rope scaling {name} {x}")
+        return x
+
+    s = positive("factor")
     if kind == "linear":
         return f / s, 1.0
     if kind == "ntk":
         if rot_dim <= 2:
             raise ValueError("ntk scaling needs rot_dim > 2")
         return (float(theta) * s ** (rot_dim / (rot_dim - 2.0))) ** (-2.0 * i / rot_dim), 1.0
-    length = float(scaling["original_length"])
+    length = positive("original_length")
     turns = length * f / (2.0 * math.pi)  # of each pair over the original length
     if kind == "yarn":
         if theta == 1.0:
             raise ValueError("yarn scaling needs theta != 1")
-        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        fast, slow = positive("beta_fast", 32.0), positive("beta_slow", 1.0)
 
         def pair_of(n):  # the (fractional) pair that turns n times
             return rot_dim * math.log(length / (n * 2.0 * math.pi)) / (2.0 * math.log(theta))
@@ -94,7 +103,7 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None 
         factor = scaling.get("attention_factor")
         return f * (1.0 - ramp) + f / s * ramp, (0.1 * math.log(s) + 1.0) if factor is None else float(factor)
     lo, hi = float(scaling.get("low", 1.0)), float(scaling.get("high", 4.0))
-    if hi <= lo:
+    if not hi > lo:
         raise ValueError("bands scaling needs high > low")
     keep = np.clip((turns - lo) / (hi - lo), 0.0, 1.0)
     return f * keep + f / s * (1.0 - keep), 1.0
@@ -160,6 +169,8 @@ class Rope:
 
     def _refuse(self, name, t, shape, dtype):
         """Says what is wrong with a tensor that failed its check."""
+        if t is None:
+            raise ValueError(f"{name} is missing")
         if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{name} must be a CUDA tensor on device {self.device}")
         if t.dtype != dtype:
@@ -170,13 +181,15 @@ class Rope:
 
     def _heads(self, name, t, shape, dtype):
         """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+        if t is None:
+            self._refuse(name, t, shape, dtype)
         st = t.stride() if t.dim() == 3 else (0, 0, 0)
         if t.shape != shape or t.dtype != dtype or t.get_device() != self.device or st[2] != 1:
             self._refuse(name, t, shape, dtype)
         return t.data_ptr(), st[0], st[1]
 
     def _flat(self, name, t, n, dtype):
-        if t.shape != (n,) or t.dtype != dtype or t.get_device() != self.device or (n > 1 and t.stride(0) != 1):
+        if t is None or t.shape != (n,) or t.dtype != dtype or t.get_device() != self.device or (n > 1 and t.stride(0) != 1):
             self._refuse(name, t, (n,), dtype)
         return t.data_ptr()
 
@@ -254,7 +267,7 @@ class Rope:
             pools[i] = pool.data_ptr()
         if blocks is None:
             raise ValueError("raw pool pointers need hot_pool_blocks")
-        if bad_flag.dtype != self._i32 or bad_flag.numel() < 1 or bad_flag.get_device() != self.device:
+        if bad_flag is None or bad_flag.dtype != self._i32 or bad_flag.numel() < 1 or bad_flag.get_device() != self.device:
             raise ValueError(f"bad_flag must be an int32 CUDA tensor on device {self.device}")
         raw = _VIEWS(T, hq, hkv, self._types[dt], qv[0], kv[0], vv[0], qv[1], qv[2], kv[1], kv[2], vv[1], vv[2], pos, qw, kw,
                      eps, 0, qo[0], 0, qo[1], qo[2], 0, 0, self._flat("slots", slots, T, self._i64), pools[0], pools[1],

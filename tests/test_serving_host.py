@@ -231,3 +231,47 @@ def test_prefix_null_arguments():
 def test_indptr_refuses(bad):
     with pytest.raises(ValueError):
         _indptr("q_indptr", bad)
+
+
+@pytest.mark.parametrize("scaling", [
+    {"type": "linear"}, {"type": "yarn", "factor": 4.0}, {"type": "bands", "factor": 4.0}, {"factor": 2.0},
+    {"type": "yarn", "factor": 4.0, "original_length": 0}, {"type": "bands", "factor": 4.0, "original_length": math.nan},
+    {"type": "yarn", "factor": 4.0, "original_length": 4096, "beta_slow": 0},
+    {"type": "yarn", "factor": 4.0, "original_length": 4096, "beta_fast": -1},
+    {"type": "yarn", "factor": 4.0, "original_length": math.inf}])
+def test_frequencies_refuse_incomplete_scalings(scaling):
+    with pytest.raises(ValueError):
+        W.rope_frequencies(64, 10000.0, scaling)
+
+
+class _CpuEngine:
+    """An engine whose device is torch's number for the CPU: calls get as far as their last check of arguments."""
+    device = -1
+
+    def __init__(self, memory):
+        self.handle = ctypes.cast(memory, ctypes.c_void_p)
+
+
+@pytest.mark.parametrize("missing", ["k_out", "q_out", "positions"])
+def test_rotate_names_a_missing_argument(engine_memory, missing):
+    import torch
+    rope = W.Rope(_CpuEngine(engine_memory), head_dim=64)
+    a = dict(q=torch.zeros(2, 4, 64, dtype=torch.float16), k=torch.zeros(2, 1, 64, dtype=torch.float16),
+             positions=torch.zeros(2, dtype=torch.int32), q_out=torch.zeros(2, 4, 64, dtype=torch.float16),
+             k_out=torch.zeros(2, 1, 64, dtype=torch.float16))
+    a[missing] = None
+    with pytest.raises(ValueError, match=missing):
+        rope.rotate(**a)
+
+
+@pytest.mark.parametrize("missing", ["k", "q_out", "positions", "slots", "bad_flag"])
+def test_append_names_a_missing_argument(engine_memory, missing):
+    import torch
+    rope = W.Rope(_CpuEngine(engine_memory), head_dim=64)
+    a = dict(q=torch.zeros(2, 4, 64, dtype=torch.float16), k=torch.zeros(2, 1, 64, dtype=torch.float16), v=None,
+             positions=torch.zeros(2, dtype=torch.int32), slots=torch.zeros(2, dtype=torch.int64),
+             hot_k=torch.zeros(1, 16, 1, 64, dtype=torch.float16), hot_v=None,
+             q_out=torch.zeros(2, 4, 64, dtype=torch.float16), bad_flag=torch.zeros(1, dtype=torch.int32))
+    a[missing] = None
+    with pytest.raises(ValueError, match=missing):
+        rope.append(**a)
