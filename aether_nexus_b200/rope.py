@@ -114,6 +114,12 @@ def token_slots(refs, indptr, lens, q_indptr) -> np.ndarray:
     queries ``q_indptr[b] .. q_indptr[b+1]`` of sequence b are the tokens that
     follow its first ``lens[b]``, in the pages ``refs[indptr[b]:indptr[b+1]]``."""
     refs = np.asarray(refs, np.uint32) & np.uint32(REF_MASK)
+    B = len(lens)
+    for name, x in (("indptr", np.asarray(indptr)[:B + 1]), ("q_indptr", np.asarray(q_indptr))):
+        if x.shape != (B + 1,) or x[0] < 0 or (x[1:] < x[:-1]).any():
+            raise ValueError(f"{name} is not a non-decreasing list of an entry per sequence and one more")
+    if int(q_indptr[0]) or any(int(n) < 0 for n in lens):
+        raise ValueError("q_indptr[0] is not 0, or a length is negative")
     out = np.empty(int(q_indptr[-1]), np.int64)
     for b in range(len(lens)):
         n = int(q_indptr[b + 1]) - int(q_indptr[b])

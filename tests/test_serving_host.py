@@ -275,3 +275,18 @@ def test_append_names_a_missing_argument(engine_memory, missing):
     a[missing] = None
     with pytest.raises(ValueError, match=missing):
         rope.append(**a)
+
+
+@pytest.mark.parametrize("args", [
+    ([5, 6], [0, 2], [-3], [0, 2]),          # would count pages from the list's end
+    ([5, 6], [0, 2], [1], [1, 3]),           # token 0 belongs to no sequence
+    ([5, 6, 7], [0, 2], [1], [0, 2, 4]),     # more sequences of queries than lengths
+    ([5, 6], [0, 2], [1, 2], [0, 1, 2]),     # more lengths than page lists
+    ([5, 6], [0, 1, 2], [1, 2], [0, 2, 1]), ([5, 6], [0, 2, 1], [1, 2], [0, 1, 2]), ([5, 6], [-2, 2], [1], [0, 1])])
+def test_token_slots_refuse_what_leaves_a_slot_unset(args):
+    with pytest.raises(ValueError):
+        W.token_slots(*args)
+
+
+def test_token_slots_without_tokens():
+    assert W.token_slots([], [0, 0], [0], [0, 0]).shape == (0,)
