@@ -1897,30 +1897,33 @@ bool disjoint_rows(uint64_t T, uint64_t H, uint64_t D, uint64_t ts, uint64_t hs)
 }
 
 // What an argument covers: [T][H] pieces of D bytes, token stride ts and head
-// stride hs in bytes.  A plain range is one piece.
+// stride hs in bytes, first to last byte at lo .. hi.  A plain range is one piece.
 struct Rows {
     const char* name;
-    const void* base;
-    uint64_t T, H, D, ts, hs;
+    uint64_t lo, hi, T, H, D, ts, hs;
+    Rows(const char* what, const void* base, uint64_t tokens, uint64_t heads, uint64_t bytes, uint64_t token, uint64_t head)
+        : name(what), lo(reinterpret_cast<uintptr_t>(base)), hi(lo), T(tokens), H(heads), D(bytes), ts(token), hs(head) {
+        if (base && T && H && D) hi = lo + (T - 1) * ts + (H - 1) * hs + D;
+    }
+    // where the residues modulo m start at lo % m, this many if no more than m
+    uint64_t residues(uint64_t m) const { return (ts % m ? (T - 1) * ts : 0) + (hs % m ? (H - 1) * hs : 0) + D; }
 };
-Rows range(const char* name, const void* base, uint64_t bytes) { return Rows{name, base, base ? 1ull : 0ull, 1, bytes, 0, 0}; }
+Rows range(const char* name, const void* base, uint64_t bytes) { return Rows(name, base, 1, 1, bytes, 0, 0); }
 
-// Whether two arguments may have bytes in common: not where their ranges are
-// apart, and not where both lie in separate residues of a common stride (slices
-// of one buffer of rows or heads).
-bool share(const Rows& x, const Rows& y) {
-    if (!x.T || !x.H || !x.D || !y.T || !y.H || !y.D) return false;
-    const uint64_t a = reinterpret_cast<uintptr_t>(x.base), b = reinterpret_cast<uintptr_t>(y.base);
-    auto span = [](const Rows& r) { return (r.T - 1) * r.ts + (r.H - 1) * r.hs + r.D; };
-    if (a + span(x) <= b || b + span(y) <= a) return false;
+// Two arguments whose ranges meet: not sharing a byte where they lie in separate
+// residues of a common stride (slices of one buffer of rows or heads).
+bool interleaved(const Rows& x, const Rows& y) {
     for (const uint64_t m : {x.T > 1 ? x.ts : 0, x.H > 1 ? x.hs : 0, y.T > 1 ? y.ts : 0, y.H > 1 ? y.hs : 0}) {
         if (!m) continue;
-        // the residues start at base % m and are this many, if no more than m
-        auto residues = [m](const Rows& r) { return (r.ts % m ? (r.T - 1) * r.ts : 0) + (r.hs % m ? (r.H - 1) * r.hs : 0) + r.D; };
-        const uint64_t nx = residues(x), ny = residues(y), d = b >= a ? (b - a) % m : (m - (a - b) % m) % m;
-        if (nx <= d && ny <= m - d) return false;
+        const uint64_t nx = x.residues(m), ny = y.residues(m), d = y.lo >= x.lo ? (y.lo - x.lo) % m : (m - (x.lo - y.lo) % m) % m;
+        if (nx <= d && ny <= m - d) return true;
     }
-    return true;
+    return false;
+}
+
+// Whether two arguments may have bytes in common.
+inline bool share(const Rows& x, const Rows& y) {
+    return x.lo < y.hi && y.lo < x.hi && x.lo < x.hi && y.lo < y.hi && !interleaved(x, y);
 }
 
 int rope_output(const char* name, const void* in, uint64_t in_ts, uint64_t in_hs, const void* out, uint64_t ts,
@@ -1938,7 +1941,7 @@ int rope_output(const char* name, const void* in, uint64_t in_ts, uint64_t in_hs
 int rope_overlaps(const weaver_rope_views* v, uint64_t D, bool append) {
     const uint64_t T = v->n_tokens, Hq = v->q_heads, Hkv = v->kv_heads, w = 2 * D;
     auto heads = [&](const char* name, const void* p, uint64_t H, uint64_t ts, uint64_t hs) {
-        return Rows{name, p, p ? T : 0, H, w, T > 1 ? 2 * ts : 0, H > 1 ? 2 * hs : 0};
+        return Rows(name, p, T, H, w, T > 1 ? 2 * ts : 0, H > 1 ? 2 * hs : 0);
     };
     const uint64_t pool = v->hot_pool_blocks * kBlock * Hkv * w;
     const Rows ins[] = {heads("q", v->q, Hq, v->q_token_stride, v->q_head_stride),
@@ -1956,7 +1959,7 @@ int rope_overlaps(const weaver_rope_views* v, uint64_t D, bool append) {
         const Rows& x = outs[o];
         for (size_t i = 0; i < std::size(ins); ++i) {
             const Rows& y = ins[i];
-            if (i == o && o < 2 && x.base == y.base && x.ts == y.ts && x.hs == y.hs) continue;  // in place
+            if (i == o && o < 2 && x.lo == y.lo && x.ts == y.ts && x.hs == y.hs) continue;  // in place
             if (share(x, y)) return fail(WEAVER_ERR_INVALID_ARGUMENT, "%s overlaps %s", x.name, y.name);
         }
         for (size_t i = 0; i < o; ++i)
