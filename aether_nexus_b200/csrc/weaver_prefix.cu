@@ -284,15 +284,16 @@ __global__ void __launch_bounds__(8 * D / 4) prefix_merge_kernel(const __grid_co
 // quarter then, and it saves writing and reading two partials a row.
 constexpr uint32_t kOwnRows = 512;
 // Starting an item (query rows in, results out, the pipeline filling) in the
-// units of a token tile's cost: 16 sequences x 8 drafts run 34.9 us with 32, 35.1
-// with 40, 36.4 with 48, 36.9 with 56, 39.1 with 16; 8 x 4 drafts 22.9 to 24.6
-// with 32 to 56 and 26.5 with 16.
+// units of a token tile's cost.  8 sequences x 4 drafts run 22.6 to 23.6 us with
+// 32, 24.3 to 24.9 with 24, 26.2 to 26.9 with 16, 23.0 to 25.0 with 40 to 56; 16 x
+// 8 drafts 35.2 to 35.9, 33.2 to 33.9, 38.1 to 38.5 and 35.4 to 36.4 (two series
+// of a graph of 20 calls).
 constexpr uint32_t kItemCost = 32;
 // Lists of up to 16 rows go to the 16-row tiles, whose many small CTAs start
 // and end faster than items of the tensor-memory kernel; lists of 9 to 16 rows
 // only where they are many (more than two tiles an SM), since a few more items
-// there cost less than another kernel (8 sequences x 4 queries of 4 heads: 23
-// us on tensor memory, 31 with both; 200 sequences x 3: 129 and 94).
+// there cost less than another kernel (8 sequences x 4 queries of 4 heads: 22.6
+// us on tensor memory, 30.5 with both; 200 sequences x 3: 120.5 and 92.7).
 constexpr uint32_t kRows16 = 16, kRowsFew = 8;
 
 // The longest run of an item.  The tensor cores cut the bits below the
@@ -306,9 +307,8 @@ constexpr uint32_t kMostTiles = 512, kMostPages = 8192;
 // The length of a 16-row item, in pages: that of least makespan on `slots`
 // resident CTAs, where an item costs kStart16 rounds beside a round for every
 // four of its pages (a page per warp).  64 sequences behind one prefix, 38 MB of
-// own pages: 67.4 us a run where the item only divided the work by the slots,
-// 65.6 so (69.9 with a start of one round, the same with 3 to 12); 40 sequences,
-// 123 MB: 81.0 and 77.2.
+// own pages: 62.1 us a run so and with 3 or 12, 66.9 with a start of one round; 40
+// sequences, 123 MB: 73.7, 74.1 and 82.3.
 constexpr uint64_t kStart16 = 6;
 static uint64_t rows16_item(const std::vector<uint64_t>& tiles, uint64_t slots) {
     uint64_t longest = 1, total = 0;
@@ -452,9 +452,10 @@ void plan_prefix(const PrefixGeometry& geo, uint32_t n_sm, PrefixTables* t) {
         return it;
     };
 
-    // 16-row tiles: items of whole multiples of four pages (one per warp), three
-    // CTAs to an SM at a time.  Of the possible item lengths the one whose items
-    // end first when dealt out longest first, as the grid is.
+    // 16-row tiles: a tile is cut into equal items, at any page.  Of the possible
+    // item lengths the one whose items end first when dealt out longest first, as
+    // the grid is, three CTAs to an SM at a time (what fits with heads of 128; with
+    // heads of 64 four fit, and the lengths are those of three all the same).
     std::vector<uint64_t> sizes;
     for (const PrefixTile& T : t->tiles)
         if (t->lists[T.list].tile_rows == 16) sizes.push_back(pages(T.list));
@@ -580,7 +581,7 @@ cudaError_t launch_prefix_rows16(const PrefixArgs& a, uint32_t n_items, cudaStre
 
 cudaError_t launch_prefix_merge(const PrefixArgs& a, uint32_t max_slots, cudaStream_t s) {
     // two shares of the runs where a row has more than eight (64 sequences of 19
-    // runs: 67.7 us a run of the plan with one share, 62.7 with two, 65.6 with
+    // runs: 67.2 us a run of the plan with one share, 62.1 with two, 65.1 with
     // four, whose warps read two rows' neighbouring 16 bytes at a time and not four)
     if (max_slots > 8) return a.D == 128 ? merge<128, 2>(a, s) : merge<64, 2>(a, s);
     return a.D == 128 ? merge<128, 1>(a, s) : merge<64, 1>(a, s);

@@ -2,8 +2,9 @@
 prefixes (``weaver_prefix_*``): personas behind one system prompt, candidates
 of one question, drafts of one context.
 
-The sequences are grouped; each group's prefix pages are read once for all
-queries of the group.  Lengths are in tokens and live on the device, so one
+The sequences are grouped; each group's prefix pages are read once for 256 rows
+(queries x query heads of a kv head) of the group's queries together, and by a
+sequence with 512 rows or more for itself.  Lengths are in tokens and live on the device, so one
 plan (and one captured graph) serves a batch while its sequences grow within
 their pages.  One token per sequence, draft batches and prompt chunks may be
 mixed in one call::
@@ -110,7 +111,8 @@ class PrefixPlan:
     def views(self, *, q, hot_k, hot_v, prefix_refs=None, suffix_refs=None, prefix_lens=None, suffix_lens=None, out=None,
               part_m=None, part_l=None, part_o=None, hot_pool_blocks=None) -> bytes:
         """The C views (``weaver_prefix_views``) of CUDA tensors, kept for
-        repeated runs: ``q`` / ``out [tokens, Hq, d]`` f16, ``hot_k`` / ``hot_v
+        repeated runs (raw addresses: the tensors have to live until the last run
+        with them is over): ``q`` / ``out [tokens, Hq, d]`` f16, ``hot_k`` / ``hot_v
         [blocks, 16, Hkv, d]`` f16 (or raw pointers with ``hot_pool_blocks``),
         refs and lengths int32 or uint32, partials fp32."""
         if hot_pool_blocks is None:

@@ -527,8 +527,9 @@ WEAVER_EXPORT int weaver_rope_append(weaver_rope* rope, const weaver_rope_views*
  * Exact attention over the hot pool in token lengths.  num_seqs sequences in
  * num_groups groups of neighbours; sequence b has queries q_indptr[b] ..
  * q_indptr[b+1]-1 and pages suffix_indptr[b] .. of suffix_refs of its own,
- * and its group's pages prefix_indptr[g] .. of prefix_refs, which are read
- * once for all queries of the group.  With nq queries of its own, query j of
+ * and its group's pages prefix_indptr[g] .. of prefix_refs.  These are read once
+ * per 256 rows (queries x q heads of a kv head) of the group's queries together;
+ * a sequence with 512 rows or more reads them for itself.  With nq queries of its own, query j of
  * a sequence attends to the whole prefix and, with WEAVER_FLAG_CAUSAL, to the
  * first suffix_len - nq + 1 + j tokens of its own pages (none where that is
  * not positive; the rule of ops.metal:549), else to all of them; scale * q.K,
