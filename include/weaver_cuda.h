@@ -545,8 +545,8 @@ WEAVER_EXPORT int weaver_rope_append(weaver_rope* rope, const weaver_rope_views*
  * the outputs of other queries of that head NaN too, causally masked or not.
  * WEAVER_FLAG_PARTIALS writes (m, l, o) instead of out, as weaver_run does (l and
  * o are sums of e^(score - m); m is near the row's largest score and need not be
- * it, and -inf with l = 0 where a query sees nothing), so that a plan over cold blocks of the same queries can be merged with
- * weaver_merge_partials. */
+ * it, and -inf with l = 0 where a query sees nothing), so that a plan over cold
+ * blocks of the same queries can be merged with weaver_merge_partials. */
 typedef struct weaver_prefix_shape {
     uint32_t num_groups, num_seqs;
     uint32_t q_heads, kv_heads, head_dim; /* q_heads % kv_heads == 0; head_dim 64 or 128 */
